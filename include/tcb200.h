@@ -235,6 +235,65 @@ int tcb200_replay_end(tcb200_replay_t* replay, int timed_replays, float* elapsed
 int tcb200_assemble_shards(const void* gathered, void* out, int world, int64_t rows, int64_t total,
                            int64_t inner, tcb200_stream_t stream);
 
+/* ---- losses of a large-vocabulary head ----------------------------------------------------------------------------
+ * No counterpart in the reference, whose operator library (tc/library) ends at the layers.  These calls take their
+ * problem by value of a struct, keep no plan and no state: scratch memory is the caller's (`workspace`, 128-byte aligned, at
+ * least the bytes the query names for the current device), so calls with workspaces of their own may overlap in time, on
+ * several streams, devices and captured graphs.  Everything is enqueued on `stream` of the current device; nothing
+ * synchronises or allocates, and every call may be captured into a graph.  Sums and statistics are fp32, each output is
+ * rounded to its type once, and results do not depend on timing (no atomics on values).
+ * A kernel whose bounded wait gives up makes the outputs NaN (dW: its first element) and stores a code in *dev_status
+ * (optional). */
+enum { TCB200_F32 = 0, TCB200_F16 = 1, TCB200_BF16 = 2 };
+
+/* Softmax cross entropy of the linear layer z = X W^T, without keeping z:
+ *   lse[n] = log sum_v exp z(n,v),  loss[n] = lse[n] - z(n, target[n]),
+ *   dX = dZ W, dW = dZ^T X  with  dZ(n,v) = grad_loss[n] (exp(z(n,v) - lse[n]) - [v = target[n]]).
+ * target[n] == ignore_index: loss, lse and the row of dX are 0, the row of X is not read.  A target outside [0, V) that is
+ * not ignore_index makes loss[n], the row of dX and all of dW NaN. */
+typedef struct tcb200_linear_ce {
+  int64_t N, D, V;         /* X is [N, D], W is [V, D], target, loss and lse are [N] */
+  int64_t ldx, ldw;        /* elements between rows of X and of W (>= D); dX and dW are dense */
+  int64_t ignore_index;
+  int32_t dtype;           /* TCB200_F32 / F16 / BF16: X, W, dX, dW.  float32 is computed to fp32 accuracy (three bf16
+                              planes per operand, six products) */
+  int32_t index_bytes;     /* 4 or 8: target is int32 or int64 */
+  int32_t pack_w;          /* f16 / bf16: 1 = rows of W may start anywhere, W is copied to aligned scratch piece by piece;
+                              0 = W is read in place, which needs W 16-byte aligned and ldw a multiple of 8, else
+                              TCB200_ERR_ALIGNMENT.  float32 always packs */
+  int32_t reserved;        /* 0 */
+} tcb200_linear_ce_t;
+int tcb200_linear_ce_workspace(const tcb200_linear_ce_t* problem, int64_t* forward_bytes, int64_t* backward_bytes);
+int tcb200_linear_ce_forward(const tcb200_linear_ce_t* problem, const void* X, const void* W, const void* target,
+                             float* loss, float* lse, void* workspace, int64_t workspace_bytes, tcb200_stream_t stream,
+                             int* dev_status);
+/* grad_loss[n * grad_stride]; grad_stride 0: one value for all rows.  dX or dW may be NULL (not computed). */
+int tcb200_linear_ce_backward(const tcb200_linear_ce_t* problem, const void* X, const void* W, const void* target,
+                              const float* lse, const float* grad_loss, int64_t grad_stride, void* dX, void* dW,
+                              void* workspace, int64_t workspace_bytes, tcb200_stream_t stream, int* dev_status);
+
+/* Distillation from a teacher's K largest logits at temperature T:
+ *   q = softmax over the row's entries of teacher / T,  p = softmax over V of logits / T,
+ *   loss[n] = T^2 sum_k q_k (ln q_k - ln p(indices[n,k])),
+ *   dlogits(n,v) = T grad_loss[n] (p(v) - sum of q_k over the entries with indices[n,k] = v).
+ * An index below 0, or a teacher logit of -inf, is no entry; a row without entries has loss 0 and gradient 0 whatever its
+ * logits hold.  An index of V or more makes the row's loss and gradient NaN.  The same index twice counts twice.
+ * stats[3n], stats[3n + 1]: maximum of the row's logits and sum of exp((logits - maximum) / T); stats[3n + 2]: log sum exp
+ * of its entries' teacher logits / T (-inf: no entries, NaN: an index of V or more).  [N, 3], for the backward call. */
+#define TCB200_TOPK_MAX 4096
+typedef struct tcb200_topk_distill {
+  int64_t N, V, K;                     /* logits is [N, V], indices and teacher are [N, K], 1 <= K <= TCB200_TOPK_MAX */
+  int64_t ld_logits, ld_indices, ld_teacher; /* elements between rows; dlogits is dense */
+  float temperature;                   /* > 0, finite */
+  int32_t logits_dtype, teacher_dtype; /* TCB200_F32 / F16 / BF16 */
+  int32_t index_bytes;                 /* 4 or 8 */
+} tcb200_topk_distill_t;
+int tcb200_topk_distill_forward(const tcb200_topk_distill_t* problem, const void* logits, const void* indices,
+                                const void* teacher, float* loss, float* stats, tcb200_stream_t stream);
+int tcb200_topk_distill_backward(const tcb200_topk_distill_t* problem, const void* logits, const void* indices,
+                                 const void* teacher, const float* stats, const float* grad_loss, int64_t grad_stride,
+                                 void* dlogits, tcb200_stream_t stream);
+
 /* Writes `bytes` of a rotating pattern to `buf` on `stream`: the bench uses it to
  * evict L2 between timed launches of the small problems. */
 int tcb200_l2_flush(void* buf, size_t bytes, tcb200_stream_t stream);

@@ -19,4 +19,7 @@ def __getattr__(name):
         import importlib
         api = importlib.import_module(".api", __name__)
         return getattr(api, name)
+    if name in ("linear_cross_entropy", "topk_distillation"):
+        import importlib
+        return getattr(importlib.import_module(".losses", __name__), name)
     raise AttributeError(name)

@@ -25,6 +25,8 @@ SYMBOLS = [
     "tcb200_timer_start", "tcb200_timer_stop", "tcb200_reduce_launch_static", "tcb200_assemble_shards",
     "tcb200_status_create", "tcb200_status_destroy", "tcb200_status_check", "tcb200_selftest_wait",
     "tcb200_replay_begin", "tcb200_replay_end",
+    "tcb200_linear_ce_workspace", "tcb200_linear_ce_forward", "tcb200_linear_ce_backward",
+    "tcb200_topk_distill_forward", "tcb200_topk_distill_backward",
 ]
 
 
@@ -51,6 +53,22 @@ class Tile(ctypes.Structure):
     def __repr__(self):
         return ("Tile(variant=%d, bm=%d, bn=%d, bk=%d, stages=%d, threads=%d, split_tf32=%d, split_k=%d)"
                 % self.as_tuple())
+
+
+F32, F16, BF16 = 0, 1, 2
+TOPK_MAX = 4096
+
+
+class LinearCe(ctypes.Structure):
+    _fields_ = [("N", ctypes.c_int64), ("D", ctypes.c_int64), ("V", ctypes.c_int64), ("ldx", ctypes.c_int64),
+                ("ldw", ctypes.c_int64), ("ignore_index", ctypes.c_int64), ("dtype", ctypes.c_int32),
+                ("index_bytes", ctypes.c_int32), ("pack_w", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class TopkDistill(ctypes.Structure):
+    _fields_ = [("N", ctypes.c_int64), ("V", ctypes.c_int64), ("K", ctypes.c_int64), ("ld_logits", ctypes.c_int64),
+                ("ld_indices", ctypes.c_int64), ("ld_teacher", ctypes.c_int64), ("temperature", ctypes.c_float),
+                ("logits_dtype", ctypes.c_int32), ("teacher_dtype", ctypes.c_int32), ("index_bytes", ctypes.c_int32)]
 
 
 class Tcb200Error(RuntimeError):
@@ -96,6 +114,12 @@ def lib():
         L.tcb200_reduce_launch_static.argtypes = [ctypes.c_void_p] * 4
         L.tcb200_assemble_shards.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64,
                                              ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p]
+        V, I64 = ctypes.c_void_p, ctypes.c_int64
+        L.tcb200_linear_ce_workspace.argtypes = [ctypes.POINTER(LinearCe), ctypes.POINTER(I64), ctypes.POINTER(I64)]
+        L.tcb200_linear_ce_forward.argtypes = [ctypes.POINTER(LinearCe), V, V, V, V, V, V, I64, V, V]
+        L.tcb200_linear_ce_backward.argtypes = [ctypes.POINTER(LinearCe), V, V, V, V, V, I64, V, V, V, I64, V, V]
+        L.tcb200_topk_distill_forward.argtypes = [ctypes.POINTER(TopkDistill), V, V, V, V, V, V]
+        L.tcb200_topk_distill_backward.argtypes = [ctypes.POINTER(TopkDistill), V, V, V, V, V, I64, V, V]
         _lib = L
     return _lib
 

@@ -7,6 +7,7 @@
 
 #include "tc/aten/aten_autotuner.h"
 #include "tc/aten/aten_compiler.h"
+#include "tc/aten/aten_losses.h"
 #include "tc/core/flags.h"
 #include "tc/lang/canonicalize.h"
 
@@ -353,6 +354,28 @@ PYBIND11_MODULE(tclib, m) {
           py::list r;
           for (const auto& l : tc::matchKernels(def)) r.append(problemDict(l));
           return r;
+        });
+
+  // ---- losses of a large-vocabulary head (tc/aten/aten_losses.h); `stream`: the caller's current one ----
+  auto toStream = [](uintptr_t s) { return reinterpret_cast<tcb200_stream_t>(s); };
+  m.def("linear_cross_entropy",
+        [toStream](const at::Tensor& x, const at::Tensor& w, const at::Tensor& target, int64_t ignoreIndex, uintptr_t stream) {
+          return tc::aten::linearCrossEntropy(x, w, target, ignoreIndex, toStream(stream));
+        });
+  m.def("linear_cross_entropy_backward",
+        [toStream](const at::Tensor& x, const at::Tensor& w, const at::Tensor& target, const at::Tensor& lse,
+                   const at::Tensor& grad, int64_t ignoreIndex, bool needX, bool needW, uintptr_t stream) {
+          return tc::aten::linearCrossEntropyBackward(x, w, target, lse, grad, ignoreIndex, needX, needW, toStream(stream));
+        });
+  m.def("topk_distillation",
+        [toStream](const at::Tensor& logits, const at::Tensor& indices, const at::Tensor& teacher, double temperature,
+                   uintptr_t stream) {
+          return tc::aten::topkDistillation(logits, indices, teacher, temperature, toStream(stream));
+        });
+  m.def("topk_distillation_backward",
+        [toStream](const at::Tensor& logits, const at::Tensor& indices, const at::Tensor& teacher, const at::Tensor& stats,
+                   const at::Tensor& grad, double temperature, uintptr_t stream) {
+          return tc::aten::topkDistillationBackward(logits, indices, teacher, stats, grad, temperature, toStream(stream));
         });
 
   m.def("set_flag", [](const std::string& name, const std::string& value) {

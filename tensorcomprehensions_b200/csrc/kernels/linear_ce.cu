@@ -1,0 +1,687 @@
+// Softmax cross entropy of a linear layer over a large vocabulary, without keeping its logits.
+//
+//   z = X W^T,  lse_n = log sum_v exp z_nv,  loss_n = lse_n - z_{n, t_n}
+//   dZ_nv = g_n (exp(z_nv - lse_n) - [v = t_n]),  dX = dZ W,  dW = dZ^T X
+//
+// Forward: one pass of the pair product (pair_gemm.cuh) over the vocabulary.  A thread of its epilogue owns 128 logits of
+// a row and leaves their maximum and the sum of exp(z - maximum); a second kernel joins these per row.  The logits never reach
+// memory.  Backward, per piece of the vocabulary: the product again, with an epilogue that writes dZ of the piece; then
+// dX += dZ W and dW = dZ^T X from it.  The work is 2 N D V operations forward and 6 N D V backward on the tensor cores,
+// which bound it from a few hundred rows up; below that one pass over W does.
+//
+// Rows are compacted first: rows without a target (target == ignore_index) cost nothing, and what their X holds, infinities
+// and NaN included, is never read.  The number of rows that remain stays on the device (pg::Args::live).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math.h>
+#include <string.h>
+
+#include <mutex>
+
+#include "pair_gemm.cuh"
+
+namespace tcb200 {
+namespace pg {
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiledFn encode_fn() {
+  static std::mutex mu;
+  static EncodeTiledFn fn = nullptr;
+  std::lock_guard<std::mutex> lock(mu);
+  if (!fn) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+    else
+      (void)cudaGetLastError();
+  }
+  return fn;
+}
+
+// k-major: box of 64 columns (k) x 128 rows.  mn-major: box of 64 columns (m or n) x 64 rows (k).  Zeros out of bounds.
+int make_map(CUtensorMap* tm, const Operand& o, bool bf16, bool mn_major) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return TCB200_ERR_CUDA;
+  cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.planes};
+  const int64_t plane = o.planes > 1 ? o.plane_stride : o.rows * o.ld;
+  cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)plane * 2};
+  cuuint32_t box[3] = {kBK, (cuuint32_t)(mn_major ? kBK : kHalf), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                  const_cast<void*>(o.base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? TCB200_OK : TCB200_ERR_CUDA;
+}
+
+}  // namespace pg
+
+namespace {
+
+using pg::kTile;
+
+// What the kernels share besides the operands, at the head of the workspace.
+struct Head {
+  int live;      // rows with a target
+  int status;    // a bounded wait that gave up
+  float gscale;  // largest |g| of the live rows
+};
+
+// ---- rows -----------------------------------------------------------------------------------------------------------
+struct Rows {
+  Head* head;
+  int* source;    // [n_pad] live row -> row
+  int* place;     // [n] row -> live row, -1 without a target
+  int* target;    // [n_pad] of a live row; -1: outside [0, V)
+  float* share;   // [n_pad] g of a live row / gscale (backward)
+  float* lse;     // [n_pad] of a live row (backward)
+};
+
+// One block walks over the rows in order: the order of the live rows, and with it every later sum, does not depend on timing.
+template <typename Index>
+__global__ void __launch_bounds__(1024) rows_kernel(const Index* target, int64_t n, int64_t v, int64_t ignore,
+                                                    const float* g, int64_t g_stride, const float* lse, Rows r) {
+  __shared__ int warp_count[32];
+  __shared__ float warp_max[32];
+  pdl_sync();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int base = 0;
+  float top = 0.f;
+  for (int64_t i0 = 0; i0 < n; i0 += 1024) {
+    const int64_t i = i0 + threadIdx.x;
+    const int64_t t = i < n ? (int64_t)target[i] : ignore;
+    const bool live = i < n && t != ignore;
+    const unsigned votes = __ballot_sync(0xffffffffu, live);
+    if (lane == 0) warp_count[warp] = __popc(votes);
+    __syncthreads();
+    int before = base, all = 0;
+    for (int w = 0; w < 32; ++w) {
+      if (w < warp) before += warp_count[w];
+      all += warp_count[w];
+    }
+    const int at = before + __popc(votes & ((1u << lane) - 1));
+    if (live) {
+      r.source[at] = (int)i;
+      r.target[at] = t >= 0 && t < v ? (int)t : -1;
+      if (g) {
+        const float x = g[i * g_stride];
+        r.share[at] = x;
+        r.lse[at] = lse[i];
+        const float ax = fabsf(x);
+        if (ax <= 3.402823466e38f) top = fmaxf(top, ax);  // the largest finite one: not NaN, not infinite
+      }
+    }
+    if (i < n) r.place[i] = live ? at : -1;
+    base += all;
+    __syncthreads();
+  }
+  if (g) {
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) warp_max[warp] = top;
+    __syncthreads();
+    for (int w = 0; w < 32; ++w) top = fmaxf(top, warp_max[w]);
+    // dZ is kept with g / max|g|: where all rows share one g, as under a mean, that is exactly 1 and the rounding
+    // of dZ to 16 bits does not meet g's significand
+    for (int i = threadIdx.x; i < base; i += 1024) {
+      const float x = r.share[i];
+      r.share[i] = r.target[i] < 0 ? __int_as_float(0x7fffffff) : (top > 0.f ? x / top : x);
+    }
+  }
+  if (threadIdx.x == 0) {
+    r.head->live = base;
+    r.head->status = 0;
+    r.head->gscale = top > 0.f ? top : 1.f;
+  }
+}
+
+// ---- operands -------------------------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ float to_float(T v);
+template <> __device__ __forceinline__ float to_float(float v) { return v; }
+template <> __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+
+__device__ __forceinline__ uint16_t bits(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
+__device__ __forceinline__ uint16_t bits(__half v) { return __half_as_ushort(v); }
+
+// v = p0 + p1 + p2, each the bf16 nearest to what is left: 24 significand bits and more.  A value without a finite
+// remainder (infinite, NaN) is carried by p0 alone.
+__device__ __forceinline__ void split3(float v, uint16_t* p) {
+  const __nv_bfloat16 a = __float2bfloat16_rn(v);
+  float r = v - __bfloat162float(a);
+  if (!(fabsf(r) <= 3.402823466e38f)) r = 0.f;
+  const __nv_bfloat16 b = __float2bfloat16_rn(r);
+  r -= __bfloat162float(b);
+  p[0] = bits(a);
+  p[1] = bits(b);
+  p[2] = bits(__float2bfloat16_rn(r));
+}
+
+// Rows of X or W as operand planes [planes][rows_cap][dp], dp = d rounded up to 8, the padding zero.  `source` picks live
+// rows: those behind the last one, up to a whole tile, are zero.  A thread makes eight columns; the input is read once.
+template <typename T>
+__global__ void __launch_bounds__(256) pack_kernel(const T* in, int64_t ld, int64_t rows, int64_t d, int64_t dp,
+                                                   const int* source, const int* live, uint16_t* out, int64_t plane) {
+  pdl_sync();
+  const bool f32 = sizeof(T) == 4;
+  const int64_t per_row = dp / 8;
+  const int64_t have = live ? *live : rows;
+  const int64_t total = (live ? (have + kTile - 1) / kTile * kTile : rows) * per_row;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / per_row, c = (i % per_row) * 8;
+    alignas(16) T v[8];
+    memset(v, 0, sizeof(v));
+    if (r < have) {
+      const T* src = in + (source ? (int64_t)source[r] : r) * ld + c;
+      if (c + 8 <= d && ((uintptr_t)src & 15) == 0) {
+#pragma unroll
+        for (int q = 0; q < (int)sizeof(T) / 2; ++q)
+          reinterpret_cast<uint4*>(v)[q] = __ldg(reinterpret_cast<const uint4*>(src) + q);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c + j < d) v[j] = src[j];
+      }
+    }
+    uint16_t* dst = out + r * dp + c;
+    if (f32) {
+      alignas(16) uint16_t w[3][8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint16_t p[3];
+        split3(to_float(v[j]), p);
+        w[0][j] = p[0]; w[1][j] = p[1]; w[2][j] = p[2];
+      }
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4*>(dst + p * plane) = *reinterpret_cast<uint4*>(w[p]);
+    } else {
+      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(v);
+    }
+  }
+}
+
+// ---- epilogues ------------------------------------------------------------------------------------------------------
+constexpr float kLog2e = 1.4426950408889634f;
+
+// exp(x), x <= 0: the base-2 exponential of the hardware; the product rounds x log2(e) to 2^-24 of itself
+__device__ __forceinline__ float exp_neg(float x) { return exp2f(x * kLog2e); }
+
+// Forward: maximum and sum of exp(z - maximum) over this thread's columns, and the target's logit.
+struct ForwardEpi {
+  const Head* head;
+  const int* target;
+  float2* part;      // [parts][n_pad]
+  float* hit;        // [n_pad] the target's logit
+  int64_t n_pad, v0, v, part0;  // first vocabulary entry of this launch, entries of it; number of its first part
+  __device__ void operator()(float (&acc)[128], int64_t row, int64_t col0, int) const {
+    if (row >= head->live || col0 >= v) return;
+    const int have = (int)min(v - col0, (int64_t)128);
+    const int64_t at = (int64_t)target[row] - v0 - col0;
+    const int t = at >= 0 && at < have ? (int)at : -1;
+    float top = -INFINITY, z = 0.f;
+#pragma unroll
+    for (int j = 0; j < 128; ++j) {
+      if (j >= have) acc[j] = -INFINITY;
+      top = fmaxf(top, acc[j]);
+      if (j == t) z = acc[j];
+    }
+    // all -inf: the sum is empty, and -inf - -inf would make NaN of it
+    const float shift = top == -INFINITY ? 0.f : top;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 128; ++j) sum[j & 3] += exp_neg(acc[j] - shift);
+    part[(part0 + col0 / 128) * n_pad + row] = make_float2(top, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+    if (t >= 0) hit[row] = z;
+  }
+};
+
+// Joins the parts of a row: lse, and the loss lse - z_target.  32 rows x 8 parts a block; a row's parts are added in a
+// fixed order.
+__global__ void __launch_bounds__(256) join_kernel(Rows r, const float2* part, const float* hit, int64_t parts,
+                                                   int64_t n_pad, int64_t n, float* loss, float* lse, int* dev_status) {
+  pdl_sync();
+  if (dev_status && r.head->status && blockIdx.x == 0 && threadIdx.x + threadIdx.y == 0)
+    atomicCAS(dev_status, 0, r.head->status);
+  __shared__ float2 share[8][33];
+  const int64_t i = blockIdx.x * 32 + threadIdx.x;
+  const int64_t at = i < n ? r.place[i] : -1;
+  float top = -INFINITY, sum = 0.f;
+  if (at >= 0) {
+    for (int64_t p = threadIdx.y; p < parts; p += 8) {
+      const float2 x = part[p * n_pad + at];
+      // fmaxf drops a NaN maximum; its sum is NaN then too and survives
+      const float m = fmaxf(top, x.x), shift = m == -INFINITY ? 0.f : m;
+      sum = sum * exp_neg(top - shift) + x.y * exp_neg(x.x - shift);
+      top = m;
+    }
+  }
+  share[threadIdx.y][threadIdx.x] = make_float2(top, sum);
+  __syncthreads();
+  if (threadIdx.y != 0 || i >= n) return;
+  for (int k = 1; k < 8; ++k) {
+    const float2 x = share[k][threadIdx.x];
+    const float m = fmaxf(top, x.x), shift = m == -INFINITY ? 0.f : m;
+    sum = sum * exp_neg(top - shift) + x.y * exp_neg(x.x - shift);
+    top = m;
+  }
+  const float nan = __int_as_float(0x7fffffff);
+  float l = top + logf(sum), e = 0.f;
+  if (at < 0) l = 0.f;
+  else if (r.target[at] < 0) e = nan;  // a target outside the vocabulary
+  else e = (top - hit[at]) + logf(sum);
+  if (r.head->status) l = e = nan;     // a wait gave up: no number is better than a wrong one
+  loss[i] = e;
+  lse[i] = l;
+}
+
+// dZ of a piece, as operand planes [planes][n_pad][ld].  f16 values carry 2^14: probabilities from 2^-28 up then keep all
+// of their 11 bits (1 / 2^-14 is f16's smallest normal number), and |dZ| <= 2^14 stays in range.
+constexpr float kHalfScale = 16384.f;
+enum { kF32 = 0, kF16 = 1, kBF16 = 2 };
+
+template <int TYPE>
+struct GradEpi {
+  const Head* head;
+  const int* target;
+  const float* share;
+  const float* lse;
+  uint16_t* out;
+  int64_t ld, plane, v0, v;
+  __device__ void operator()(float (&acc)[128], int64_t row, int64_t col0, int) const {
+    if (col0 >= ld) return;
+    const bool live = row < head->live;
+    const float g = live ? share[row] : 0.f, l = live ? lse[row] : 0.f;
+    const int64_t at = live ? (int64_t)target[row] - v0 - col0 : -1;
+    const int t = at >= 0 && at < 128 ? (int)at : -1;
+    const int have = live ? (int)min(v - col0, (int64_t)128) : 0;
+    uint16_t* dst = out + row * ld + col0;
+#pragma unroll
+    for (int c = 0; c < 128; c += 8) {
+      alignas(16) uint16_t w[3][8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float d = acc[c + j] - l;
+        const float p = TYPE == kF32 ? expf(d) : exp_neg(d);
+        const float x = c + j < have ? g * (c + j == t ? p - 1.f : p) : 0.f;
+        if (TYPE == kF32) {
+          uint16_t s[3];
+          split3(x, s);
+          w[0][j] = s[0]; w[1][j] = s[1]; w[2][j] = s[2];
+        } else {
+          w[0][j] = TYPE == kF16 ? bits(__float2half_rn(x * kHalfScale)) : bits(__float2bfloat16_rn(x));
+        }
+      }
+      if (col0 + c < ld) {
+#pragma unroll
+        for (int p = 0; p < (TYPE == kF32 ? 3 : 1); ++p)
+          *reinterpret_cast<uint4*>(dst + p * plane + c) = *reinterpret_cast<uint4*>(w[p]);
+      }
+    }
+  }
+};
+
+// dX of a piece: fp32 sums, one plane per split of the piece, added to over the pieces.
+struct SumEpi {
+  float* out;  // [splits][n_pad][ld], ld a multiple of 8
+  int64_t ld, plane;
+  int add;
+  __device__ void operator()(float (&acc)[128], int64_t row, int64_t col0, int split) const {
+    float* dst = out + split * plane + row * ld + col0;
+#pragma unroll
+    for (int c = 0; c < 128; c += 4)
+      if (col0 + c < ld) {
+        float4* p = reinterpret_cast<float4*>(dst + c);
+        float4 o = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+        if (add) {
+          const float4 old = *p;
+          o.x += old.x; o.y += old.y; o.z += old.z; o.w += old.w;
+        }
+        *p = o;
+      }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+
+// dW of a piece: whole sums, scaled and rounded once.
+template <typename T>
+struct WeightEpi {
+  const Head* head;
+  T* out;
+  int64_t ld, rows, d;
+  float scale;
+  int vec;  // rows start on 16-byte boundaries
+  __device__ void operator()(float (&acc)[128], int64_t row, int64_t col0, int) const {
+    if (row >= rows || col0 >= d) return;
+    const float k = head->gscale * scale;
+    T* dst = out + row * ld + col0;
+    constexpr int W = 16 / sizeof(T);
+#pragma unroll
+    for (int c = 0; c < 128; c += W) {
+      alignas(16) T w[W];
+#pragma unroll
+      for (int j = 0; j < W; ++j) w[j] = from_float<T>(acc[c + j] * k);
+      if (vec && col0 + c + W <= d) {
+        *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<uint4*>(w);
+      } else {
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+          if (col0 + c + j < d) dst[c + j] = w[j];
+      }
+    }
+  }
+};
+
+// dX: the splits' sums added in order, scaled, rounded once and put back in the rows' places; zero where a row has no target.
+template <typename T>
+__global__ void __launch_bounds__(256) finish_kernel(Rows r, const float* sums, int splits, int64_t plane, int64_t ld,
+                                                     int64_t n, int64_t d, float scale, T* dx, T* dw,
+                                                     int* dev_status) {
+  pdl_sync();
+  if (dev_status && r.head->status && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(dev_status, 0, r.head->status);
+  const float nan = __int_as_float(0x7fffffff);
+  const bool bad = r.head->status != 0;  // a wait gave up somewhere: the gradients say so
+  if (bad && dw && blockIdx.x == 0 && threadIdx.x == 0) dw[0] = from_float<T>(nan);
+  if (!dx) return;
+  const float k = r.head->gscale * scale;
+  const int64_t per_row = ld / 8;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n * per_row; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t row = i / per_row, c = (i % per_row) * 8;
+    const int at = r.place[row];
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (at >= 0) {
+      for (int s = 0; s < splits; ++s) {
+        const float4* p = reinterpret_cast<const float4*>(sums + s * plane + at * ld + c);
+        const float4 a = p[0], b = p[1];
+        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+        v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+      }
+    }
+    T* dst = dx + row * d + c;
+    alignas(16) T w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = from_float<T>(bad ? nan : (at >= 0 ? v[j] * k : 0.f));
+    if (c + 8 <= d && ((uintptr_t)dst & 15) == 0) {
+#pragma unroll
+      for (int q = 0; q < (int)sizeof(T) / 2; ++q) reinterpret_cast<uint4*>(dst)[q] = reinterpret_cast<uint4*>(w)[q];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < d) dst[j] = w[j];
+    }
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+constexpr int64_t kPieceBytes = 256ll << 20;  // dZ of a piece, and a packed piece of W
+
+struct Layout {
+  int64_t n_pad, dp, planes;
+  int64_t fwd_piece, bwd_piece;  // vocabulary entries per piece
+  int64_t parts;
+  int splits;
+  int64_t fwd_bytes, bwd_bytes;
+  // byte offsets
+  int64_t source, place, target, share, lse, hit, part, x, w_fwd, w_bwd, dz, sums;
+};
+
+bool pack_w(const tcb200_linear_ce_t& p) { return p.dtype == TCB200_F32 || p.pack_w; }
+
+int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
+  if (!q) return TCB200_ERR_INVALID_ARGUMENT;
+  const tcb200_linear_ce_t& p = *q;
+  if (p.N < 0 || p.D < 1 || p.V < 1 || p.ldx < p.D || p.ldw < p.D) return TCB200_ERR_INVALID_ARGUMENT;
+  if (p.dtype != TCB200_F32 && p.dtype != TCB200_F16 && p.dtype != TCB200_BF16) return TCB200_ERR_INVALID_ARGUMENT;
+  if (p.index_bytes != 4 && p.index_bytes != 8) return TCB200_ERR_INVALID_ARGUMENT;
+  const int64_t limit = (1ll << 31) - 1024;
+  if (p.N > limit || p.V > limit || p.D > (1ll << 20) || p.ldw > (1ll << 38) || p.ldx > (1ll << 38)) return TCB200_ERR_TOO_LARGE;
+  if (!pack_w(p) && p.ldw % 8 != 0) return TCB200_ERR_ALIGNMENT;
+  l->n_pad = round_up(std::max<int64_t>(p.N, 1), kTile);
+  l->dp = round_up(p.D, 8);
+  l->planes = p.dtype == TCB200_F32 ? 3 : 1;
+  const int64_t v_pad = round_up(p.V, kTile);
+  // A packed piece of W, and dZ of a piece, take at most 256 MiB where that leaves 4096 entries a piece; pieces are even.
+  auto piece = [&](int64_t bytes_per_entry) {
+    const int64_t most = std::max<int64_t>(kPieceBytes / bytes_per_entry / kTile * kTile, 16 * kTile);
+    const int64_t pieces = ceil_div(v_pad, most);
+    return round_up(ceil_div(v_pad, pieces), kTile);
+  };
+  l->fwd_piece = pack_w(p) ? piece(l->dp * 2 * l->planes) : v_pad;
+  l->bwd_piece = piece(2 * l->planes * (pack_w(p) ? std::max(l->dp, l->n_pad) : l->n_pad));
+  l->parts = ceil_div(p.V, 128);
+  // few tiles of dX: the vocabulary of a piece is split so that the pairs of the device have one unit each
+  const int64_t tiles = (l->n_pad / kTile) * ceil_div(p.D, kTile);
+  const int64_t kb = ceil_div(l->bwd_piece, pg::kBK);
+  l->splits = (int)std::max<int64_t>(1, std::min<int64_t>((sms / 2) / tiles, kb / 4));
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += round_up(std::max<int64_t>(bytes, 16), 1024);
+    return here;
+  };
+  take(sizeof(Head));
+  l->source = take(l->n_pad * 4);
+  l->place = take(p.N * 4);
+  l->target = take(l->n_pad * 4);
+  l->share = take(l->n_pad * 4);
+  l->lse = take(l->n_pad * 4);
+  l->x = take(l->planes * l->n_pad * l->dp * 2);
+  const int64_t common = at;
+  l->hit = take(l->n_pad * 4);
+  l->part = take(l->parts * l->n_pad * 8);
+  l->w_fwd = take(pack_w(p) ? l->planes * l->fwd_piece * l->dp * 2 : 0);
+  l->fwd_bytes = at;
+  at = common;
+  l->w_bwd = take(pack_w(p) ? l->planes * l->bwd_piece * l->dp * 2 : 0);
+  l->dz = take(l->planes * l->n_pad * l->bwd_piece * 2);
+  l->sums = take((int64_t)l->splits * l->n_pad * l->dp * 4);
+  l->bwd_bytes = at;
+  return TCB200_OK;
+}
+
+Rows rows_of(char* ws, const Layout& l) {
+  Rows r;
+  r.head = reinterpret_cast<Head*>(ws);
+  r.source = reinterpret_cast<int*>(ws + l.source);
+  r.place = reinterpret_cast<int*>(ws + l.place);
+  r.target = reinterpret_cast<int*>(ws + l.target);
+  r.share = reinterpret_cast<float*>(ws + l.share);
+  r.lse = reinterpret_cast<float*>(ws + l.lse);
+  return r;
+}
+
+int launch_rows(const tcb200_linear_ce_t& p, const void* target, const float* g, int64_t g_stride, const float* lse,
+                const Rows& r, cudaStream_t s) {
+  if (p.index_bytes == 8)
+    TCB200_CUDA_TRY(launch_pdl(rows_kernel<int64_t>, dim3(1), dim3(1024), 0, s, static_cast<const int64_t*>(target), p.N,
+                               p.V, p.ignore_index, g, g_stride, lse, r));
+  else
+    TCB200_CUDA_TRY(launch_pdl(rows_kernel<int32_t>, dim3(1), dim3(1024), 0, s, static_cast<const int32_t*>(target), p.N,
+                               p.V, p.ignore_index, g, g_stride, lse, r));
+  return TCB200_OK;
+}
+
+int launch_pack(const tcb200_linear_ce_t& p, const Layout& l, const void* in, int64_t ld, int64_t rows, const int* source,
+                const int* live, void* out, int64_t plane, int sms, cudaStream_t s) {
+  const int64_t items = (live ? l.n_pad : rows) * (l.dp / 8);
+  const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(items, 256), 8ll * sms)));
+  uint16_t* o = static_cast<uint16_t*>(out);
+  cudaError_t e;
+  if (p.dtype == TCB200_F32)
+    e = launch_pdl(pack_kernel<float>, grid, dim3(256), 0, s, static_cast<const float*>(in), ld, rows, p.D, l.dp, source, live, o, plane);
+  else  // f16 and bf16 are copied as they are
+    e = launch_pdl(pack_kernel<__half>, grid, dim3(256), 0, s, static_cast<const __half*>(in), ld, rows, p.D, l.dp, source, live, o, plane);
+  TCB200_CUDA_TRY(e);
+  return TCB200_OK;
+}
+
+size_t elem_bytes(const tcb200_linear_ce_t& p) { return p.dtype == TCB200_F32 ? 4 : 2; }
+
+pg::Args gemm_args(const Layout& l, int64_t M, int64_t N, int64_t K, const int* live, int live_is_k, int* status) {
+  pg::Args a = {};
+  a.M = M;
+  a.N = N;
+  a.K = K;
+  a.live = live;
+  a.live_is_k = live_is_k;
+  a.products = l.planes == 3 ? 6 : 1;
+  // a drain every 512 k (32 MMAs), 256 k of float32 operands (16 MMAs of the largest planes after 80 of smaller ones):
+  // the truncation of the tensor core's sums then stays near 2^-20 of a term's size
+  a.chunk_kb = l.planes == 3 ? 4 : 8;
+  a.splits = 1;
+  a.dev_status = status;
+  return a;
+}
+
+// The operand of entries [v0, v0 + v) of W: in place, or packed into `packed`.
+int w_operand(const tcb200_linear_ce_t& p, const Layout& l, const void* W, int64_t v0, int64_t v, int64_t piece, void* packed,
+              int sms, cudaStream_t s, pg::Operand* o) {
+  const char* base = static_cast<const char*>(W) + (size_t)v0 * p.ldw * elem_bytes(p);
+  if (!pack_w(p)) {
+    *o = {base, p.D, v, p.ldw, 1, 0};
+    return TCB200_OK;
+  }
+  *o = {packed, l.dp, v, l.dp, l.planes, piece * l.dp};
+  return launch_pack(p, l, base, p.ldw, v, nullptr, nullptr, packed, piece * l.dp, sms, s);
+}
+
+int current_device(int* device) {
+  TCB200_CUDA_TRY(cudaGetDevice(device));
+  return TCB200_OK;
+}
+
+template <typename T, int TYPE>
+int backward_typed(const tcb200_linear_ce_t& p, const Layout& l, const void* W, const Rows& r, char* ws, T* dX, T* dW,
+                   int device, int sms, cudaStream_t s, int* status, int* dev_status) {
+  const bool bf16 = TYPE != kF16;
+  const float scale = TYPE == kF16 ? 1.f / kHalfScale : 1.f;
+  const pg::Operand x{ws + l.x, l.dp, l.n_pad, l.dp, l.planes, l.n_pad * l.dp};
+  float* sums = reinterpret_cast<float*>(ws + l.sums);
+  int st;
+  for (int64_t v0 = 0; v0 < p.V; v0 += l.bwd_piece) {
+    const int64_t v = std::min(l.bwd_piece, p.V - v0), ld = l.bwd_piece;
+    pg::Operand w;
+    if ((st = w_operand(p, l, W, v0, v, l.bwd_piece, ws + l.w_bwd, sms, s, &w)) != TCB200_OK) return st;
+    uint16_t* dz = reinterpret_cast<uint16_t*>(ws + l.dz);
+    const GradEpi<TYPE> ge{r.head, r.target, r.share, r.lse, dz, ld, l.n_pad * ld, v0, v};
+    st = pg::launch<false, false>(x, w, bf16, gemm_args(l, p.N, v, p.D, &r.head->live, 0, status), ge, device, sms, s);
+    if (st != TCB200_OK) return st;
+    const pg::Operand z{dz, v, l.n_pad, ld, l.planes, l.n_pad * ld};
+    if (dX) {
+      const SumEpi se{sums, l.dp, l.n_pad * l.dp, v0 > 0};
+      pg::Args a = gemm_args(l, p.N, p.D, v, &r.head->live, 0, status);
+      a.splits = l.splits;
+      a.split_kb = (int)ceil_div(ceil_div(v, pg::kBK), l.splits);
+      if ((st = pg::launch<false, true>(z, w, bf16, a, se, device, sms, s)) != TCB200_OK) return st;
+    }
+    if (dW) {
+      T* out = dW + v0 * p.D;
+      const int vec = (p.D * sizeof(T)) % 16 == 0 && ((uintptr_t)out & 15) == 0;
+      const WeightEpi<T> we{r.head, out, p.D, v, p.D, scale, vec};
+      st = pg::launch<true, true>(z, x, bf16, gemm_args(l, v, p.D, p.N, &r.head->live, 1, status), we, device, sms, s);
+      if (st != TCB200_OK) return st;
+    }
+  }
+  const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(p.N * (l.dp / 8), 256), 8ll * sms)));
+  TCB200_CUDA_TRY(launch_pdl(finish_kernel<T>, grid, dim3(256), 0, s, r, static_cast<const float*>(sums), l.splits,
+                             l.n_pad * l.dp, l.dp, p.N, p.D, scale, dX, dW, dev_status));
+  return TCB200_OK;
+}
+
+}  // namespace
+}  // namespace tcb200
+
+using namespace tcb200;
+
+extern "C" {
+
+int tcb200_linear_ce_workspace(const tcb200_linear_ce_t* problem, int64_t* forward_bytes, int64_t* backward_bytes) {
+  Layout l;
+  const int st = layout_of(problem, sm_count(-1), &l);
+  if (st != TCB200_OK) return st;
+  if (forward_bytes) *forward_bytes = l.fwd_bytes;
+  if (backward_bytes) *backward_bytes = l.bwd_bytes;
+  return TCB200_OK;
+}
+
+int tcb200_linear_ce_forward(const tcb200_linear_ce_t* problem, const void* X, const void* W, const void* target,
+                             float* loss, float* lse, void* workspace, int64_t workspace_bytes, tcb200_stream_t stream,
+                             int* dev_status) {
+  Layout l;
+  int device, st = layout_of(problem, sm_count(-1), &l);
+  if (st != TCB200_OK) return st;
+  const tcb200_linear_ce_t& p = *problem;
+  if (p.N == 0) return TCB200_OK;
+  if (!X || !W || !target || !loss || !lse || !workspace) return TCB200_ERR_INVALID_ARGUMENT;
+  if (workspace_bytes < l.fwd_bytes) return TCB200_ERR_INVALID_ARGUMENT;
+  if (((uintptr_t)workspace & 127) || (!pack_w(p) && ((uintptr_t)W & 15))) return TCB200_ERR_ALIGNMENT;
+  if ((st = current_device(&device)) != TCB200_OK) return st;
+  const int sms = sm_count(device);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  const Rows r = rows_of(ws, l);
+  int* status = &r.head->status;
+  if ((st = launch_rows(p, target, nullptr, 0, nullptr, r, s)) != TCB200_OK) return st;
+  st = launch_pack(p, l, X, p.ldx, p.N, r.source, &r.head->live, ws + l.x, l.n_pad * l.dp, sms, s);
+  if (st != TCB200_OK) return st;
+  const pg::Operand x{ws + l.x, l.dp, l.n_pad, l.dp, l.planes, l.n_pad * l.dp};
+  float2* part = reinterpret_cast<float2*>(ws + l.part);
+  float* hit = reinterpret_cast<float*>(ws + l.hit);
+  for (int64_t v0 = 0; v0 < p.V; v0 += l.fwd_piece) {
+    const int64_t v = std::min(l.fwd_piece, p.V - v0);
+    pg::Operand w;
+    if ((st = w_operand(p, l, W, v0, v, l.fwd_piece, ws + l.w_fwd, sms, s, &w)) != TCB200_OK) return st;
+    const ForwardEpi e{r.head, r.target, part, hit, l.n_pad, v0, v, v0 / 128};
+    st = pg::launch<false, false>(x, w, p.dtype != TCB200_F16, gemm_args(l, p.N, v, p.D, &r.head->live, 0, status), e,
+                                  device, sms, s);
+    if (st != TCB200_OK) return st;
+  }
+  TCB200_CUDA_TRY(launch_pdl(join_kernel, dim3((unsigned)ceil_div(p.N, 32)), dim3(32, 8), 0, s, r,
+                             static_cast<const float2*>(part), static_cast<const float*>(hit), l.parts, l.n_pad, p.N, loss, lse, dev_status));
+  return TCB200_OK;
+}
+
+int tcb200_linear_ce_backward(const tcb200_linear_ce_t* problem, const void* X, const void* W, const void* target,
+                              const float* lse, const float* grad_loss, int64_t grad_stride, void* dX, void* dW,
+                              void* workspace, int64_t workspace_bytes, tcb200_stream_t stream, int* dev_status) {
+  Layout l;
+  int device, st = layout_of(problem, sm_count(-1), &l);
+  if (st != TCB200_OK) return st;
+  const tcb200_linear_ce_t& p = *problem;
+  if (!dX && !dW) return TCB200_OK;
+  if (grad_stride < 0) return TCB200_ERR_INVALID_ARGUMENT;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (p.N == 0) {  // no rows: dX is empty, dW the empty sum
+    if (dW) TCB200_CUDA_TRY(cudaMemsetAsync(dW, 0, (size_t)p.V * p.D * elem_bytes(p), s));
+    return TCB200_OK;
+  }
+  if (!X || !W || !target || !lse || !grad_loss || !workspace) return TCB200_ERR_INVALID_ARGUMENT;
+  if (workspace_bytes < l.bwd_bytes) return TCB200_ERR_INVALID_ARGUMENT;
+  if (((uintptr_t)workspace & 127) || (!pack_w(p) && ((uintptr_t)W & 15))) return TCB200_ERR_ALIGNMENT;
+  if ((st = current_device(&device)) != TCB200_OK) return st;
+  const int sms = sm_count(device);
+  char* ws = static_cast<char*>(workspace);
+  const Rows r = rows_of(ws, l);
+  int* status = &r.head->status;
+  if ((st = launch_rows(p, target, grad_loss, grad_stride, lse, r, s)) != TCB200_OK) return st;
+  st = launch_pack(p, l, X, p.ldx, p.N, r.source, &r.head->live, ws + l.x, l.n_pad * l.dp, sms, s);
+  if (st != TCB200_OK) return st;
+  switch (p.dtype) {
+    case TCB200_F32:
+      return backward_typed<float, kF32>(p, l, W, r, ws, static_cast<float*>(dX), static_cast<float*>(dW), device, sms, s, status, dev_status);
+    case TCB200_F16:
+      return backward_typed<__half, kF16>(p, l, W, r, ws, static_cast<__half*>(dX), static_cast<__half*>(dW), device, sms, s, status, dev_status);
+    default:
+      return backward_typed<__nv_bfloat16, kBF16>(p, l, W, r, ws, static_cast<__nv_bfloat16*>(dX), static_cast<__nv_bfloat16*>(dW),
+                                                  device, sms, s, status, dev_status);
+  }
+}
+
+}  // extern "C"

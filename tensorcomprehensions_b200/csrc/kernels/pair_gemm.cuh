@@ -1,0 +1,311 @@
+// 16-bit matrix products on CTA pairs with fp32 accuracy of the sum, shared by the kernels of the large-vocabulary
+// losses (sm_100a).  One pair computes a 256 x 256 tile C(m, n) = sum_k A(m, k) B(n, k); the epilogue is a functor that
+// gets a row and 128 consecutive columns of it in registers.
+//
+// Operands are f16 or bf16 (both the same), each either k-major (rows of k) or mn-major (rows of m or n): the three
+// products of a linear layer's training step (X W^T, dZ W, dZ^T X) then read the same arrays without a transposed copy.
+// float32 operands arrive as three bf16 planes a = a0 + a1 + a2 (8 + 8 + 8 significand bits); of the nine plane products
+// the six with i + j <= 2 are summed, smallest first, and the largest dropped one is 2^-24 of the product.
+//
+// Roles of a CTA (10 warps): warps 0-7 drain the accumulator and run the epilogue, warp 8 issues the TMA loads of this CTA's
+// 128 rows of A and 128 of the tile's 256 rows of B, one thread of the leader's warp 9 issues the MMAs (M = 256, N = 256,
+// K = 16) of both CTAs.  The tensor core adds into its accumulator with truncation, so a sum of hundreds of MMAs drifts
+// (about half an ulp each, all the same way); the accumulator is therefore drained every `chunk_kb` k-blocks into registers
+// and the chunks are added there with rounding to nearest.  Two accumulators of 256 columns alternate, so the drain of one
+// runs under the MMAs of the other.
+#pragma once
+
+#include "common.cuh"
+#include "tcgen05.cuh"
+
+namespace tcb200 {
+namespace pg {
+
+constexpr int kTile = 256;      // tile rows and columns of a pair
+constexpr int kHalf = 128;      // rows of A, and of B, that one CTA loads
+constexpr int kBK = 64;         // k of a stage: one 128-byte swizzle row of 16-bit values
+constexpr int kOperandBytes = kHalf * kBK * 2;
+constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kStages = 6;
+constexpr int kDrainWarps = 8;
+constexpr int kThreads = (kDrainWarps + 2) * 32;
+constexpr int kBarrierBytes = 256;
+constexpr int kSmemBytes = kStages * kStageBytes + kBarrierBytes + 1024;
+static_assert(kSmemBytes <= 227 * 1024, "the stages exceed shared memory");
+constexpr int kMaxProducts = 6;
+
+struct Args {
+  int64_t M, N, K;          // extents; one of them may be replaced by *live
+  const int* live;          // null, or a device count that replaces M (live_is_k = 0) or K (live_is_k = 1)
+  int live_is_k;
+  int products;             // plane products per k-block: 1, or 6 for float32
+  int pa[kMaxProducts], pb[kMaxProducts];
+  int chunk_kb;             // k-blocks per drain
+  int splits, split_kb;     // the reduction's k-blocks go to `splits` units of split_kb each
+  uint32_t idesc;           // instruction descriptor
+  int* dev_status;
+};
+
+// Loads whose completion is counted on a barrier of either CTA of the pair: the peer's loads arrive on the leader's.
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* tm, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3, %4}], [%5];" ::"r"(smem_u32(dst)),
+      "l"(tm), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t map_to_rank(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void umma_f16_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Shared-memory descriptors, 128-byte swizzle.  k-major: rows of 64 k, 8-row groups 1024 bytes apart.  mn-major: groups of 64
+// m (or n) of 64 k-rows of 128 bytes each; 8-row groups of k 1024 bytes apart, groups of 64 m kBK * 128 bytes apart.
+template <bool MN>
+__device__ __forceinline__ uint64_t operand_desc(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
+  d |= (uint64_t)(MN ? (kBK * 128) >> 4 : 1) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;  // descriptor version of sm_100
+  d |= (uint64_t)2 << 61;  // 128-byte swizzle
+  return d;
+}
+// bytes from one MMA's k (16) to the next within a stage
+template <bool MN>
+__host__ __device__ constexpr uint32_t k_step_bytes() { return MN ? 16 * 128 : 32; }
+
+// kind::f16: D = f32, A = B = f16 (bf16 = 0) or bf16, each k-major or mn-major.
+__host__ inline uint32_t make_idesc(bool bf16, bool a_mn, bool b_mn) {
+  const uint32_t t = bf16 ? 1 : 0;
+  return (1u << 4) | (t << 7) | (t << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
+         ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+}
+
+// One operand stage of this CTA: 128 rows of m (or n) from mn0, 64 k from k0.
+template <bool MN>
+__device__ __forceinline__ void load_operand(uint8_t* dst, const CUtensorMap* tm, int mn0, int k0, int plane, uint32_t bar) {
+  if (MN) {
+    tma_load_3d_pair(dst, tm, mn0, k0, plane, bar);
+    tma_load_3d_pair(dst + kBK * 128, tm, mn0 + 64, k0, plane, bar);
+  } else {
+    tma_load_3d_pair(dst, tm, k0, mn0, plane, bar);
+  }
+}
+
+// A unit is (tile, split).  Tiles are taken in groups of 8 tile rows, rows fastest inside a group: the pairs that run at the
+// same time then share rows of B (8 pairs each) and of A, which the L2 serves.
+struct Units {
+  int64_t tiles_m, tiles_n, units;
+  int kb, splits, split_kb;
+  __device__ Units(const Args& a) {
+    int64_t M = a.M, K = a.K;
+    if (a.live) (a.live_is_k ? K : M) = *a.live;
+    tiles_m = (M + kTile - 1) / kTile;
+    tiles_n = (a.N + kTile - 1) / kTile;
+    kb = (int)((K + kBK - 1) / kBK);
+    splits = a.splits;
+    split_kb = a.split_kb > 0 ? a.split_kb : kb;
+    units = tiles_m * tiles_n * splits;
+  }
+  __device__ void locate(int64_t u, int64_t* tm, int64_t* tn, int* split, int* kb0, int* nkb) const {
+    const int64_t tiles = tiles_m * tiles_n;
+    *split = (int)(u / tiles);
+    int64_t t = u % tiles;
+    const int64_t per_group = 8 * tiles_n, g = t / per_group;
+    const int64_t rows = tiles_m - g * 8 < 8 ? tiles_m - g * 8 : 8;
+    t -= g * per_group;
+    *tm = g * 8 + t % rows;
+    *tn = t / rows;
+    *kb0 = *split * split_kb;
+    const int left = kb - *kb0;
+    *nkb = left < 0 ? 0 : (left < split_kb ? left : split_kb);
+  }
+};
+
+// Epi: struct with  __device__ void operator()(float (&acc)[128], int64_t row, int64_t col0, int split)  where row and col0
+// are the thread's row and first column of C (both may lie outside it).
+template <bool A_MN, bool B_MN, class Epi>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                 const __grid_constant__ Args a, const __grid_constant__ Epi epi) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);  // used in the leader: both CTAs' loads
+  uint64_t* empty = full + kStages;
+  uint64_t* acc_full = empty + kStages;   // [2]
+  uint64_t* acc_empty = acc_full + 2;     // [2], used in the leader: sixteen drain warps
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert((2 * kStages + 4) * 8 + 8 <= kBarrierBytes, "barrier area");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int64_t pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 2 * kDrainWarps);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kDrainWarps + 1) tmem_alloc_pair(tmem_slot, 512);
+  tc_fence_before();
+  cluster_sync_all();
+  tc_fence_after();
+  pdl_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  const Units units(a);
+
+  if (warp == kDrainWarps) {
+    // ------------------------------------------------ TMA producer
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int64_t u = pair; u < units.units && ok; u += num_pairs) {
+        int64_t tm, tn;
+        int split, kb0, nkb;
+        units.locate(u, &tm, &tn, &split, &kb0, &nkb);
+        const int m0 = (int)(tm * kTile) + (int)rank * kHalf, n0 = (int)(tn * kTile) + (int)rank * kHalf;
+        for (int c0 = 0; c0 < nkb && ok; c0 += a.chunk_kb) {
+          const int c1 = c0 + a.chunk_kb < nkb ? c0 + a.chunk_kb : nkb;
+          for (int p = 0; p < a.products && ok; ++p)
+            for (int kb = c0; kb < c1; ++kb, ++it) {
+              const int s = it % kStages;
+              ok = mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1, 21, a.dev_status, abort_flag);
+              if (!ok) break;
+              if (rank == 0) mbar_expect_tx(&full[s], 2 * kStageBytes);
+              const uint32_t bar = map_to_rank(&full[s], 0);
+              load_operand<A_MN>(smem + s * kStageBytes, &tmA, m0, (kb0 + kb) * kBK, a.pa[p], bar);
+              load_operand<B_MN>(smem + s * kStageBytes + kOperandBytes, &tmB, n0, (kb0 + kb) * kBK, a.pb[p], bar);
+            }
+        }
+      }
+    }
+  } else if (warp == kDrainWarps + 1) {
+    // ------------------------------------------------ MMA issuer
+    if (lane == 0 && rank == 0) {
+      uint32_t it = 0, chunk = 0;
+      bool ok = true;
+      for (int64_t u = pair; u < units.units && ok; u += num_pairs) {
+        int64_t tm, tn;
+        int split, kb0, nkb;
+        units.locate(u, &tm, &tn, &split, &kb0, &nkb);
+        for (int c0 = 0; c0 < nkb && ok; c0 += a.chunk_kb, ++chunk) {
+          const int c1 = c0 + a.chunk_kb < nkb ? c0 + a.chunk_kb : nkb;
+          const int steps = (c1 - c0) * a.products;
+          const int b = chunk & 1;
+          ok = mbar_wait(&acc_empty[b], ((chunk >> 1) & 1) ^ 1, 22, a.dev_status, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          uint32_t accumulate = 0;
+          for (int i = 0; i < steps; ++i, ++it) {
+            const int s = it % kStages;
+            ok = mbar_wait(&full[s], (it / kStages) & 1, 23, a.dev_status, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t sa = smem_u32(smem + s * kStageBytes), sb = sa + kOperandBytes;
+#pragma unroll
+            for (int k = 0; k < kBK / 16; ++k) {
+              umma_f16_pair(tmem_base + b * kTile, operand_desc<A_MN>(sa + k * k_step_bytes<A_MN>()),
+                            operand_desc<B_MN>(sb + k * k_step_bytes<B_MN>()), a.idesc, accumulate);
+              accumulate = 1;
+            }
+            umma_commit_pair(&empty[s]);
+          }
+          if (!ok) break;
+          umma_commit_pair(&acc_full[b]);
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------ drain + epilogue
+    const int q = warp & 3, half = warp >> 2;  // tensor-memory lane quarter; which 128 of the 256 columns
+    const uint32_t lane_base = (uint32_t)(q * 32) << 16;
+    uint32_t chunk = 0;
+    bool ok = true;
+    for (int64_t u = pair; u < units.units && ok; u += num_pairs) {
+      int64_t tm, tn;
+      int split, kb0, nkb;
+      units.locate(u, &tm, &tn, &split, &kb0, &nkb);
+      float acc[128];
+#pragma unroll
+      for (int j = 0; j < 128; ++j) acc[j] = 0.f;
+      for (int c0 = 0; c0 < nkb; c0 += a.chunk_kb, ++chunk) {
+        const int b = chunk & 1;
+        ok = mbar_wait(&acc_full[b], (chunk >> 1) & 1, 24, a.dev_status, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+          float v[16];
+          tmem_ld16_nowait(tmem_base + b * kTile + lane_base + half * 128 + g * 16, v);
+          tmem_wait_ld();
+          if (g == 7) {
+            tc_fence_before();
+            mbar_arrive_warp_remote(&acc_empty[b], 0);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[g * 16 + j] += v[j];
+        }
+      }
+      if (!ok) break;
+      epi(acc, tm * kTile + (int64_t)rank * kHalf + q * 32 + lane, tn * kTile + half * 128, split);
+    }
+  }
+
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync_all();  // no CTA leaves (or frees tensor memory) while its peer may still use it
+  if (warp == kDrainWarps + 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+// One operand: [planes][rows][cols] 16-bit values, rows `ld` apart (ld * 2 and the base multiples of 16).
+struct Operand {
+  const void* base;
+  int64_t cols, rows, ld, planes, plane_stride;
+};
+int make_map(CUtensorMap* tm, const Operand& o, bool bf16, bool mn_major);
+
+template <bool A_MN, bool B_MN, class Epi>
+int launch(const Operand& A, const Operand& B, bool bf16, Args args, const Epi& epi, int device, int sms, cudaStream_t s) {
+  CUtensorMap ta, tb;
+  int st = make_map(&ta, A, bf16, A_MN);
+  if (st == TCB200_OK) st = make_map(&tb, B, bf16, B_MN);
+  if (st != TCB200_OK) return st;
+  args.idesc = make_idesc(bf16, A_MN, B_MN);
+  if (args.products == 1) args.pa[0] = args.pb[0] = 0;
+  else {
+    const int pa[6] = {2, 1, 0, 1, 0, 0}, pb[6] = {0, 1, 2, 0, 1, 0};
+    for (int i = 0; i < 6; ++i) args.pa[i] = pa[i], args.pb[i] = pb[i];
+  }
+  const int64_t units = ceil_div(args.M, kTile) * ceil_div(args.N, kTile) * args.splits;
+  if (units == 0) return TCB200_OK;
+  const unsigned pairs = (unsigned)std::min<int64_t>(units, std::max(1, sms / 2));
+  static std::atomic<uint64_t> configured{0};
+  TCB200_CUDA_TRY(ensure_dynamic_smem(pair_gemm_kernel<A_MN, B_MN, Epi>, kSmemBytes, device, configured));
+  TCB200_CUDA_TRY(launch_pdl(pair_gemm_kernel<A_MN, B_MN, Epi>, dim3(2 * pairs), dim3(kThreads), kSmemBytes, s, ta, tb, args, epi));
+  return TCB200_OK;
+}
+
+}  // namespace pg
+}  // namespace tcb200

@@ -1,0 +1,83 @@
+"""What the losses refuse, and what their C entry points say of a problem, without a device."""
+import ctypes
+
+import pytest
+import torch
+
+import tensorcomprehensions_b200 as tc
+from tensorcomprehensions_b200 import cabi
+
+PTR = ctypes.c_void_p(1 << 20)  # never dereferenced: the calls fail before any work
+
+
+def ce(N=100, D=64, V=1000, ldx=None, ldw=None, dtype=cabi.BF16, index_bytes=8, pack_w=0):
+    return cabi.LinearCe(N, D, V, D if ldx is None else ldx, D if ldw is None else ldw, -100, dtype, index_bytes, pack_w, 0)
+
+
+def workspace(p):
+    f, b = ctypes.c_int64(), ctypes.c_int64()
+    return cabi.lib().tcb200_linear_ce_workspace(ctypes.byref(p), ctypes.byref(f), ctypes.byref(b)), f.value, b.value
+
+
+def test_workspace_follows_the_problem_and_stays_far_below_the_logits():
+    st, f, b = workspace(ce())
+    assert st == 0 and 0 < f < b
+    # 8192 x 131072: the logits would take 2 GiB in 16 bits; the forward pass keeps 8 bytes per 128 of them
+    st, f, b = workspace(ce(8192, 4096, 131072))
+    assert st == 0 and f < (200 << 20) and b < (640 << 20)
+    assert workspace(ce(8192, 4096, 131072, pack_w=1))[1] > f
+    assert workspace(ce(100, 64, 1000, dtype=cabi.F32))[2] > workspace(ce(100, 64, 1000))[2]
+    assert workspace(ce(0))[0] == 0
+
+
+def test_linear_ce_argument_checks():
+    for bad in (dict(N=-1), dict(D=0), dict(V=0), dict(ldx=63), dict(ldw=63), dict(dtype=3), dict(dtype=-1), dict(index_bytes=2)):
+        assert workspace(ce(**bad))[0] == -1, bad
+    assert workspace(ce(D=65))[0] == -4                      # rows of W off their 16-byte boundaries, not packed
+    assert workspace(ce(D=65, pack_w=1))[0] == 0
+    assert workspace(ce(D=65, dtype=cabi.F32))[0] == 0       # always packed
+    assert workspace(ce(V=1 << 31))[0] == -7 and workspace(ce(D=1 << 21))[0] == -7
+    L, p = cabi.lib(), ce()
+    _, f, b = workspace(p)
+    assert L.tcb200_linear_ce_workspace(None, None, None) == -1
+    r = ctypes.byref(p)
+    assert L.tcb200_linear_ce_forward(r, None, PTR, PTR, PTR, PTR, PTR, f, None, None) == -1
+    assert L.tcb200_linear_ce_forward(r, PTR, PTR, PTR, PTR, PTR, PTR, f - 1, None, None) == -1
+    assert L.tcb200_linear_ce_forward(r, PTR, PTR, PTR, PTR, PTR, ctypes.c_void_p((1 << 20) + 16), f, None, None) == -4
+    assert L.tcb200_linear_ce_forward(r, PTR, ctypes.c_void_p((1 << 20) + 2), PTR, PTR, PTR, PTR, f, None, None) == -4
+    assert L.tcb200_linear_ce_backward(r, PTR, PTR, PTR, PTR, PTR, -1, PTR, PTR, PTR, b, None, None) == -1
+    assert L.tcb200_linear_ce_backward(r, PTR, PTR, PTR, PTR, None, 1, PTR, PTR, PTR, b, None, None) == -1
+    assert L.tcb200_linear_ce_backward(r, PTR, PTR, PTR, PTR, PTR, 1, PTR, PTR, PTR, b - 1, None, None) == -1
+    assert L.tcb200_linear_ce_backward(r, PTR, PTR, PTR, PTR, PTR, 1, None, None, None, 0, None, None) == 0   # nothing asked for
+    assert L.tcb200_linear_ce_forward(ctypes.byref(ce(0)), None, PTR, None, None, None, None, 0, None, None) == 0
+
+
+def kd(N=10, V=1000, K=8, ldl=None, ldi=None, ldt=None, temperature=1.0, dtype=cabi.BF16, teacher=cabi.BF16, index_bytes=8):
+    return cabi.TopkDistill(N, V, K, V if ldl is None else ldl, K if ldi is None else ldi, K if ldt is None else ldt, temperature, dtype, teacher, index_bytes)
+
+
+def test_topk_distill_argument_checks():
+    L = cabi.lib()
+
+    def call(p):
+        r = ctypes.byref(p)
+        # a null among the pointers: a problem that passes its own checks is refused for it, before any launch
+        f = L.tcb200_topk_distill_forward(r, PTR, PTR, PTR, PTR, None, None)
+        assert f == L.tcb200_topk_distill_backward(r, PTR, PTR, PTR, PTR, PTR, 1, None, None)
+        return f
+
+    assert call(kd()) == -1
+    assert call(kd(N=0)) == 0
+    for bad in (dict(N=-1), dict(V=0), dict(K=0), dict(ldl=999), dict(ldi=7), dict(ldt=7), dict(dtype=9), dict(teacher=-1), dict(index_bytes=1),
+                dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=float("inf")), dict(temperature=float("nan"))):
+        assert call(kd(**{"N": 0, **bad})) == -1, bad      # N = 0 would succeed if the check let it through
+    assert call(kd(N=0, K=cabi.TOPK_MAX + 1)) == -7 and call(kd(N=0, V=1 << 31)) == -7 and call(kd(N=1 << 27)) == -7
+    assert L.tcb200_topk_distill_forward(None, PTR, PTR, PTR, PTR, PTR, None) == -1
+
+
+def test_tensors_off_the_device_are_refused():
+    x, w, t = torch.zeros(4, 8), torch.zeros(16, 8), torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="X must be a CUDA tensor"):
+        tc.linear_cross_entropy(x, w, t)
+    with pytest.raises(RuntimeError, match="logits must be a CUDA tensor"):
+        tc.topk_distillation(torch.zeros(4, 16), torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, 2))
