@@ -58,6 +58,21 @@ int make_map(CUtensorMap* tm, const Operand& o, bool bf16, bool mn_major) {
   return r == CUDA_SUCCESS ? TCB200_OK : TCB200_ERR_CUDA;
 }
 
+int make_out_map(CUtensorMap* tm, const Operand& o, int bytes) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return TCB200_ERR_CUDA;
+  cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.planes};
+  const int64_t plane = o.planes > 1 ? o.plane_stride : o.rows * o.ld;
+  cuuint64_t strides[2] = {(cuuint64_t)(o.ld * bytes), (cuuint64_t)(plane * bytes)};
+  cuuint32_t box[3] = {(cuuint32_t)(128 / bytes), 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  // 16-bit words move as they are
+  CUresult r = fn(tm, bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                  const_cast<void*>(o.base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? TCB200_OK : TCB200_ERR_CUDA;
+}
+
 }  // namespace pg
 
 namespace {
@@ -216,7 +231,7 @@ struct ForwardEpi {
   float2* part;      // [parts][n_pad]
   float* hit;        // [n_pad] the target's logit
   int64_t n_pad, v0, v, part0;  // first vocabulary entry of this launch, entries of it; number of its first part
-  __device__ void operator()(float (&acc)[128], int64_t row, int64_t col0, int) const {
+  __device__ void operator()(float (&acc)[128], int row, int col0, int, const CUtensorMap*, const pg::Out&) const {
     if (row >= head->live || col0 >= v) return;
     const int have = (int)min(v - col0, (int64_t)128);
     const int64_t at = (int64_t)target[row] - v0 - col0;
@@ -288,36 +303,43 @@ struct GradEpi {
   const int* target;
   const float* share;
   const float* lse;
-  uint16_t* out;
-  int64_t ld, plane, v0, v;
-  __device__ void operator()(float (&acc)[128], int64_t row, int64_t col0, int) const {
+  int64_t ld, v0, v;
+  __device__ void operator()(float (&acc)[128], int row, int col0, int, const CUtensorMap* tm, const pg::Out& out) const {
     if (col0 >= ld) return;
     const bool live = row < head->live;
     const float g = live ? share[row] : 0.f, l = live ? lse[row] : 0.f;
     const int64_t at = live ? (int64_t)target[row] - v0 - col0 : -1;
     const int t = at >= 0 && at < 128 ? (int)at : -1;
     const int have = live ? (int)min(v - col0, (int64_t)128) : 0;
-    uint16_t* dst = out + row * ld + col0;
 #pragma unroll
-    for (int c = 0; c < 128; c += 8) {
-      alignas(16) uint16_t w[3][8];
+    for (int c = 0; c < 128; ++c) {
+      const float d = acc[c] - l;
+      const float p = TYPE == kF32 ? expf(d) : exp_neg(d);
+      acc[c] = c < have ? g * (c == t ? p - 1.f : p) : 0.f;
+    }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float d = acc[c + j] - l;
-        const float p = TYPE == kF32 ? expf(d) : exp_neg(d);
-        const float x = c + j < have ? g * (c + j == t ? p - 1.f : p) : 0.f;
-        if (TYPE == kF32) {
-          uint16_t s[3];
-          split3(x, s);
-          w[0][j] = s[0]; w[1][j] = s[1]; w[2][j] = s[2];
-        } else {
-          w[0][j] = TYPE == kF16 ? bits(__float2half_rn(x * kHalfScale)) : bits(__float2bfloat16_rn(x));
+    for (int p = 0; p < (TYPE == kF32 ? 3 : 1); ++p) {
+#pragma unroll
+      for (int h = 0; h < 128; h += 64) {  // a box: 64 columns
+        out.begin();
+#pragma unroll
+        for (int c = 0; c < 64; c += 8) {
+          alignas(16) uint16_t w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float& x = acc[h + c + j];
+            if (TYPE == kF16) {
+              w[j] = bits(__float2half_rn(x * kHalfScale));
+            } else {
+              const __nv_bfloat16 b = __float2bfloat16_rn(x);
+              w[j] = bits(b);
+              // what is left for the next plane; a value that is not finite is carried by the first plane alone
+              if (TYPE == kF32) x = fabsf(x) <= 3.0e38f ? x - __bfloat162float(b) : 0.f;
+            }
+          }
+          out.put(c / 8, *reinterpret_cast<uint4*>(w));
         }
-      }
-      if (col0 + c < ld) {
-#pragma unroll
-        for (int p = 0; p < (TYPE == kF32 ? 3 : 1); ++p)
-          *reinterpret_cast<uint4*>(dst + p * plane + c) = *reinterpret_cast<uint4*>(w[p]);
+        out.send(tm, col0 + h, row - out.lane, p);
       }
     }
   }
@@ -325,22 +347,20 @@ struct GradEpi {
 
 // dX of a piece: fp32 sums, one plane per split of the piece, added to over the pieces.
 struct SumEpi {
-  float* out;  // [splits][n_pad][ld], ld a multiple of 8
-  int64_t ld, plane;
+  int64_t ld;  // columns of the sums
   int add;
-  __device__ void operator()(float (&acc)[128], int64_t row, int64_t col0, int split) const {
-    float* dst = out + split * plane + row * ld + col0;
+  __device__ void operator()(float (&acc)[128], int row, int col0, int split, const CUtensorMap* tm, const pg::Out& out) const {
 #pragma unroll
-    for (int c = 0; c < 128; c += 4)
-      if (col0 + c < ld) {
-        float4* p = reinterpret_cast<float4*>(dst + c);
-        float4 o = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
-        if (add) {
-          const float4 old = *p;
-          o.x += old.x; o.y += old.y; o.z += old.z; o.w += old.w;
-        }
-        *p = o;
-      }
+    for (int h = 0; h < 128; h += 32) {
+      if (col0 + h >= ld) return;
+      out.begin();
+#pragma unroll
+      for (int c = 0; c < 32; c += 4)
+        out.put(c / 4, make_uint4(__float_as_uint(acc[h + c]), __float_as_uint(acc[h + c + 1]), __float_as_uint(acc[h + c + 2]),
+                                  __float_as_uint(acc[h + c + 3])));
+      if (add) out.send_add(tm, col0 + h, row - out.lane, split);
+      else out.send(tm, col0 + h, row - out.lane, split);
+    }
   }
 };
 
@@ -354,26 +374,37 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { retur
 template <typename T>
 struct WeightEpi {
   const Head* head;
-  T* out;
-  int64_t ld, rows, d;
+  T* dst;
+  int64_t rows, d;
   float scale;
-  int vec;  // rows start on 16-byte boundaries
-  __device__ void operator()(float (&acc)[128], int64_t row, int64_t col0, int) const {
-    if (row >= rows || col0 >= d) return;
+  int tma;  // rows start on 16-byte boundaries
+  __device__ void operator()(float (&acc)[128], int row, int col0, int, const CUtensorMap* tm, const pg::Out& out) const {
+    const int row0 = row - out.lane;
+    if (row0 >= rows) return;
     const float k = head->gscale * scale;
-    T* dst = out + row * ld + col0;
-    constexpr int W = 16 / sizeof(T);
+    constexpr int W = 16 / sizeof(T), COLS = 128 / sizeof(T);
 #pragma unroll
-    for (int c = 0; c < 128; c += W) {
-      alignas(16) T w[W];
+    for (int h = 0; h < 128; h += COLS) {
+      if (col0 + h >= d) return;
+      out.begin();
 #pragma unroll
-      for (int j = 0; j < W; ++j) w[j] = from_float<T>(acc[c + j] * k);
-      if (vec && col0 + c + W <= d) {
-        *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<uint4*>(w);
-      } else {
+      for (int c = 0; c < COLS; c += W) {
+        alignas(16) T w[W];
 #pragma unroll
-        for (int j = 0; j < W; ++j)
-          if (col0 + c + j < d) dst[c + j] = w[j];
+        for (int j = 0; j < W; ++j) w[j] = from_float<T>(acc[h + c + j] * k);
+        out.put(c / W, *reinterpret_cast<uint4*>(w));
+      }
+      if (tma) {
+        out.send(tm, col0 + h, row0, 0);
+      } else {  // lane by lane along a row
+        __syncwarp();
+        const int have = (int)min(rows - row0, (int64_t)32);
+        for (int r = 0; r < have; ++r)
+#pragma unroll
+          for (int c = 0; c < COLS; c += 32)
+            if (col0 + h + c + out.lane < d)
+              dst[(row0 + r) * d + col0 + h + c + out.lane] = *static_cast<const T*>(out.at(r, c + out.lane, sizeof(T)));
+        __syncwarp();
       }
     }
   }
@@ -456,10 +487,20 @@ int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
   l->fwd_piece = pack_w(p) ? piece(l->dp * 2 * l->planes) : v_pad;
   l->bwd_piece = piece(2 * l->planes * (pack_w(p) ? std::max(l->dp, l->n_pad) : l->n_pad));
   l->parts = ceil_div(p.V, 128);
-  // few tiles of dX: the vocabulary of a piece is split so that the pairs of the device have one unit each
-  const int64_t tiles = (l->n_pad / kTile) * ceil_div(p.D, kTile);
-  const int64_t kb = ceil_div(l->bwd_piece, pg::kBK);
-  l->splits = (int)std::max<int64_t>(1, std::min<int64_t>((sms / 2) / tiles, kb / 4));
+  // dX has few tiles and a long sum: the vocabulary of a piece is split where that fills the last round of the pairs.
+  // Cost of S splits in k-blocks of a pair: rounds x (a unit's k-blocks + 8 for its start and epilogue) + what adding S
+  // planes costs (a plane of a tile is about 4 k-blocks of memory traffic).
+  const int64_t tiles = (l->n_pad / kTile) * ceil_div(p.D, kTile), pairs = std::max(1, sms / 2);
+  const int64_t kb = ceil_div(l->bwd_piece, pg::kBK) * (l->planes == 3 ? 6 : 1);
+  int64_t best = INT64_MAX;
+  l->splits = 1;
+  for (int64_t s = 1; s <= 64 && s * 8 <= kb; ++s) {
+    const int64_t cost = ceil_div(tiles * s, pairs) * (ceil_div(kb, s) + 8) + s * (9 * tiles / pairs + 1);
+    if (cost < best) {
+      best = cost;
+      l->splits = (int)s;
+    }
+  }
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t here = at;
@@ -524,7 +565,8 @@ int launch_pack(const tcb200_linear_ce_t& p, const Layout& l, const void* in, in
 
 size_t elem_bytes(const tcb200_linear_ce_t& p) { return p.dtype == TCB200_F32 ? 4 : 2; }
 
-pg::Args gemm_args(const Layout& l, int64_t M, int64_t N, int64_t K, const int* live, int live_is_k, int* status) {
+// `forward`: the loss keeps fp32 accuracy whatever the inputs' type.
+pg::Args gemm_args(const Layout& l, int64_t M, int64_t N, int64_t K, const int* live, int live_is_k, int* status, bool forward) {
   pg::Args a = {};
   a.M = M;
   a.N = N;
@@ -532,9 +574,11 @@ pg::Args gemm_args(const Layout& l, int64_t M, int64_t N, int64_t K, const int* 
   a.live = live;
   a.live_is_k = live_is_k;
   a.products = l.planes == 3 ? 6 : 1;
-  // a drain every 512 k (32 MMAs), 256 k of float32 operands (16 MMAs of the largest planes after 80 of smaller ones):
-  // the truncation of the tensor core's sums then stays near 2^-20 of a term's size
-  a.chunk_kb = l.planes == 3 ? 4 : 8;
+  // A drain every 512 k (32 MMAs), 256 k of float32 operands (16 MMAs of the largest planes after 80 of smaller ones): the
+  // truncation of the tensor core's sums then stays near 2^-20 of a term's size.  Gradients that are rounded to 16 bits
+  // in the end take 1024 k: half as many drains, which leaves the epilogues twice the time before they hold up the MMAs
+  // (dZ of 4096 x 2048 x 32000: 414 -> 350 us).
+  a.chunk_kb = l.planes == 3 ? 4 : forward ? 8 : 16;
   a.splits = 1;
   a.dev_status = status;
   return a;
@@ -570,22 +614,27 @@ int backward_typed(const tcb200_linear_ce_t& p, const Layout& l, const void* W, 
     pg::Operand w;
     if ((st = w_operand(p, l, W, v0, v, l.bwd_piece, ws + l.w_bwd, sms, s, &w)) != TCB200_OK) return st;
     uint16_t* dz = reinterpret_cast<uint16_t*>(ws + l.dz);
-    const GradEpi<TYPE> ge{r.head, r.target, r.share, r.lse, dz, ld, l.n_pad * ld, v0, v};
-    st = pg::launch<false, false>(x, w, bf16, gemm_args(l, p.N, v, p.D, &r.head->live, 0, status), ge, device, sms, s);
+    const GradEpi<TYPE> ge{r.head, r.target, r.share, r.lse, ld, v0, v};
+    CUtensorMap tc;
+    if ((st = pg::make_out_map(&tc, {dz, ld, l.n_pad, ld, l.planes, l.n_pad * ld}, 2)) != TCB200_OK) return st;
+    st = pg::launch<false, false>(x, w, bf16, gemm_args(l, p.N, v, p.D, &r.head->live, 0, status, false), tc, ge, device, sms, s);
     if (st != TCB200_OK) return st;
     const pg::Operand z{dz, v, l.n_pad, ld, l.planes, l.n_pad * ld};
     if (dX) {
-      const SumEpi se{sums, l.dp, l.n_pad * l.dp, v0 > 0};
-      pg::Args a = gemm_args(l, p.N, p.D, v, &r.head->live, 0, status);
+      const SumEpi se{l.dp, v0 > 0};
+      st = pg::make_out_map(&tc, {sums, l.dp, l.n_pad, l.dp, l.splits, l.n_pad * l.dp}, 4);
+      if (st != TCB200_OK) return st;
+      pg::Args a = gemm_args(l, p.N, p.D, v, &r.head->live, 0, status, false);
       a.splits = l.splits;
       a.split_kb = (int)ceil_div(ceil_div(v, pg::kBK), l.splits);
-      if ((st = pg::launch<false, true>(z, w, bf16, a, se, device, sms, s)) != TCB200_OK) return st;
+      if ((st = pg::launch<false, true>(z, w, bf16, a, tc, se, device, sms, s)) != TCB200_OK) return st;
     }
     if (dW) {
       T* out = dW + v0 * p.D;
-      const int vec = (p.D * sizeof(T)) % 16 == 0 && ((uintptr_t)out & 15) == 0;
-      const WeightEpi<T> we{r.head, out, p.D, v, p.D, scale, vec};
-      st = pg::launch<true, true>(z, x, bf16, gemm_args(l, v, p.D, p.N, &r.head->live, 1, status), we, device, sms, s);
+      const int tma = (p.D * sizeof(T)) % 16 == 0 && ((uintptr_t)out & 15) == 0;
+      if (tma && (st = pg::make_out_map(&tc, {out, p.D, v, p.D, 1, 0}, sizeof(T))) != TCB200_OK) return st;
+      const WeightEpi<T> we{r.head, out, v, p.D, scale, tma};
+      st = pg::launch<true, true>(z, x, bf16, gemm_args(l, v, p.D, p.N, &r.head->live, 1, status, false), tc, we, device, sms, s);
       if (st != TCB200_OK) return st;
     }
   }
@@ -639,8 +688,8 @@ int tcb200_linear_ce_forward(const tcb200_linear_ce_t* problem, const void* X, c
     pg::Operand w;
     if ((st = w_operand(p, l, W, v0, v, l.fwd_piece, ws + l.w_fwd, sms, s, &w)) != TCB200_OK) return st;
     const ForwardEpi e{r.head, r.target, part, hit, l.n_pad, v0, v, v0 / 128};
-    st = pg::launch<false, false>(x, w, p.dtype != TCB200_F16, gemm_args(l, p.N, v, p.D, &r.head->live, 0, status), e,
-                                  device, sms, s);
+    st = pg::launch<false, false>(x, w, p.dtype != TCB200_F16, gemm_args(l, p.N, v, p.D, &r.head->live, 0, status, true),
+                                  CUtensorMap{}, e, device, sms, s);
     if (st != TCB200_OK) return st;
   }
   TCB200_CUDA_TRY(launch_pdl(join_kernel, dim3((unsigned)ceil_div(p.N, 32)), dim3(32, 8), 0, s, r,

@@ -7,9 +7,13 @@
 // float32 operands arrive as three bf16 planes a = a0 + a1 + a2 (8 + 8 + 8 significand bits); of the nine plane products
 // the six with i + j <= 2 are summed, smallest first, and the largest dropped one is 2^-24 of the product.
 //
-// Roles of a CTA (10 warps): warps 0-7 drain the accumulator and run the epilogue, warp 8 issues the TMA loads of this CTA's
-// 128 rows of A and 128 of the tile's 256 rows of B, one thread of the leader's warp 9 issues the MMAs (M = 256, N = 256,
-// K = 16) of both CTAs.  The tensor core adds into its accumulator with truncation, so a sum of hundreds of MMAs drifts
+// Roles of a CTA: warps 0-7 drain the accumulator and run the epilogue, warp 8 issues the TMA loads of this CTA's
+// 128 rows of A and 128 of the tile's 256 rows of B, the leader's warp 9 issues the MMAs (M = 256, N = 256, K = 16) of both
+// CTAs.  In both issuing warps all lanes run the loop and one elected lane issues, so that descriptors and addresses stay in
+// uniform registers.  With loops that only lane 0 ran, a k-block's loads took 400 cycles to issue and its four MMAs 300, and a
+// k-block 740 cycles where its MMAs take 512 (4096 x 2048 x 32000, forward: 393 us; now 332 us, 1.62 PFLOP/s).  Of the rest
+// two issuers with half of the columns each, shorter or longer rings (4 to 6 stages) and higher boxes gained nothing.
+// The tensor core adds into its accumulator with truncation, so a sum of hundreds of MMAs drifts
 // (about half an ulp each, all the same way); the accumulator is therefore drained every `chunk_kb` k-blocks into registers
 // and the chunks are added there with rounding to nearest.  Two accumulators of 256 columns alternate, so the drain of one
 // runs under the MMAs of the other.
@@ -30,7 +34,10 @@ constexpr int kStages = 6;
 constexpr int kDrainWarps = 8;
 constexpr int kThreads = (kDrainWarps + 2) * 32;
 constexpr int kBarrierBytes = 256;
-constexpr int kSmemBytes = kStages * kStageBytes + kBarrierBytes + 1024;
+constexpr int kOutBytes = 4096;  // staging of a drain warp: 32 rows of 128 bytes
+constexpr int kOutOffset = kStages * kStageBytes;
+constexpr int kBarrierOffset = kOutOffset + kDrainWarps * kOutBytes;
+constexpr int kSmemBytes = kBarrierOffset + kBarrierBytes + 1024;
 static_assert(kSmemBytes <= 227 * 1024, "the stages exceed shared memory");
 constexpr int kMaxProducts = 6;
 
@@ -67,6 +74,11 @@ __device__ __forceinline__ void umma_f16_pair(uint32_t tmem_d, uint64_t adesc, u
       "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
 // Shared-memory descriptors, 128-byte swizzle.  k-major: rows of 64 k, 8-row groups 1024 bytes apart.  mn-major: groups of 64
 // m (or n) of 64 k-rows of 128 bytes each; 8-row groups of k 1024 bytes apart, groups of 64 m kBK * 128 bytes apart.
@@ -132,18 +144,58 @@ struct Units {
   }
 };
 
-// Epi: struct with  __device__ void operator()(float (&acc)[128], int64_t row, int64_t col0, int split)  where row and col0
-// are the thread's row and first column of C (both may lie outside it).
+// How an epilogue writes: a thread owns a row, so stores straight from its registers touch 32 rows an instruction.  Instead a
+// warp puts 32 rows x 128 bytes into its staging buffer (16-byte chunks permuted as the 128-byte swizzle does: free of
+// bank conflicts) and one lane sends the box with a TMA store, which clips at the tensor's edge.
+struct Out {
+  uint8_t* buf;
+  int lane;
+  // the previous box has left the buffer
+  __device__ __forceinline__ void begin() const {
+    if (lane == 0) tma_store_wait_read();
+    __syncwarp();
+  }
+  __device__ __forceinline__ void put(int chunk, const uint4& v) const {
+    *reinterpret_cast<uint4*>(buf + lane * 128 + ((chunk ^ (lane & 7)) << 4)) = v;
+  }
+  __device__ __forceinline__ void send(const CUtensorMap* tm, int x, int y, int z) const {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_3d(tm, buf, x, y, z);
+      tma_store_commit();
+    }
+  }
+  // the same, added to what memory holds (fp32)
+  __device__ __forceinline__ void send_add(const CUtensorMap* tm, int x, int y, int z) const {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+      asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(tm),
+                   "r"(x), "r"(y), "r"(z), "r"(smem_u32(buf))
+                   : "memory");
+      tma_store_commit();
+    }
+  }
+  // element `col` (of `bytes` bytes) of row `row`, for rows that no TMA store can address
+  __device__ __forceinline__ const void* at(int row, int col, int bytes) const {
+    const int b = col * bytes;
+    return buf + row * 128 + (((b >> 4) ^ (row & 7)) << 4) + (b & 15);
+  }
+};
+
+// Epi: struct with  __device__ void operator()(float (&acc)[128], int row, int col0, int split, const CUtensorMap* tm,
+// const Out& out)  where row and col0 are the thread's row and first column of C (both may lie outside it).
 template <bool A_MN, bool B_MN, class Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                 const __grid_constant__ Args a, const __grid_constant__ Epi epi) {
+                 const __grid_constant__ CUtensorMap tmC, const __grid_constant__ Args a, const __grid_constant__ Epi epi) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);  // used in the leader: both CTAs' loads
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kBarrierOffset);  // used in the leader: both CTAs' loads
   uint64_t* empty = full + kStages;
   uint64_t* acc_full = empty + kStages;   // [2]
-  uint64_t* acc_empty = acc_full + 2;     // [2], used in the leader: sixteen drain warps
+  uint64_t* acc_empty = acc_full + 2;     // [2], used in the leader: the drain warps of both CTAs
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   static_assert((2 * kStages + 4) * 8 + 8 <= kBarrierBytes, "barrier area");
@@ -170,37 +222,49 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   tc_fence_after();
   pdl_sync();
   const uint32_t tmem_base = *tmem_slot;
+
   const Units units(a);
 
   if (warp == kDrainWarps) {
     // ------------------------------------------------ TMA producer
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      for (int64_t u = pair; u < units.units && ok; u += num_pairs) {
-        int64_t tm, tn;
-        int split, kb0, nkb;
-        units.locate(u, &tm, &tn, &split, &kb0, &nkb);
-        const int m0 = (int)(tm * kTile) + (int)rank * kHalf, n0 = (int)(tn * kTile) + (int)rank * kHalf;
-        for (int c0 = 0; c0 < nkb && ok; c0 += a.chunk_kb) {
-          const int c1 = c0 + a.chunk_kb < nkb ? c0 + a.chunk_kb : nkb;
-          for (int p = 0; p < a.products && ok; ++p)
-            for (int kb = c0; kb < c1; ++kb, ++it) {
-              const int s = it % kStages;
-              ok = mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1, 21, a.dev_status, abort_flag);
-              if (!ok) break;
+    const bool issuer = elect_one();
+    const uint32_t full0 = map_to_rank(&full[0], 0);
+    int s = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    for (int64_t u = pair; u < units.units && ok; u += num_pairs) {
+      int64_t tm, tn;
+      int split, kb0, nkb;
+      units.locate(u, &tm, &tn, &split, &kb0, &nkb);
+      const int m0 = (int)(tm * kTile) + (int)rank * kHalf, n0 = (int)(tn * kTile) + (int)rank * kHalf;
+      for (int c0 = 0; c0 < nkb && ok; c0 += a.chunk_kb) {
+        const int c1 = c0 + a.chunk_kb < nkb ? c0 + a.chunk_kb : nkb;
+        for (int p = 0; p < a.products && ok; ++p)
+          for (int kb = c0; kb < c1; ++kb) {
+            ok = mbar_wait(&empty[s], phase, 21, a.dev_status, abort_flag);
+            if (!ok) break;
+            if (issuer) {
               if (rank == 0) mbar_expect_tx(&full[s], 2 * kStageBytes);
-              const uint32_t bar = map_to_rank(&full[s], 0);
-              load_operand<A_MN>(smem + s * kStageBytes, &tmA, m0, (kb0 + kb) * kBK, a.pa[p], bar);
-              load_operand<B_MN>(smem + s * kStageBytes + kOperandBytes, &tmB, n0, (kb0 + kb) * kBK, a.pb[p], bar);
+              uint8_t* dst = smem + s * kStageBytes;
+              load_operand<A_MN>(dst, &tmA, m0, (kb0 + kb) * kBK, a.pa[p], full0 + s * 8);
+              load_operand<B_MN>(dst + kOperandBytes, &tmB, n0, (kb0 + kb) * kBK, a.pb[p], full0 + s * 8);
             }
-        }
+            __syncwarp();
+            if (++s == kStages) {
+              s = 0;
+              phase ^= 1;
+            }
+          }
       }
     }
   } else if (warp == kDrainWarps + 1) {
     // ------------------------------------------------ MMA issuer
-    if (lane == 0 && rank == 0) {
-      uint32_t it = 0, chunk = 0;
+    if (rank == 0) {
+      const bool issuer = elect_one();
+      const uint32_t smem0 = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
+      const uint32_t tmem0 = __shfl_sync(0xffffffffu, tmem_base, 0);
+      int s = 0;
+      uint32_t phase = 0, chunk = 0;
       bool ok = true;
       for (int64_t u = pair; u < units.units && ok; u += num_pairs) {
         int64_t tm, tn;
@@ -213,23 +277,26 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           ok = mbar_wait(&acc_empty[b], ((chunk >> 1) & 1) ^ 1, 22, a.dev_status, abort_flag);
           if (!ok) break;
           tc_fence_after();
-          uint32_t accumulate = 0;
-          for (int i = 0; i < steps; ++i, ++it) {
-            const int s = it % kStages;
-            ok = mbar_wait(&full[s], (it / kStages) & 1, 23, a.dev_status, abort_flag);
+          for (int i = 0; i < steps; ++i) {
+            ok = mbar_wait(&full[s], phase, 23, a.dev_status, abort_flag);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t sa = smem_u32(smem + s * kStageBytes), sb = sa + kOperandBytes;
+            const uint32_t sa = smem0 + s * kStageBytes, sb = sa + kOperandBytes;
+            const uint64_t da = operand_desc<A_MN>(sa), db = operand_desc<B_MN>(sb);
+            if (issuer) {
 #pragma unroll
-            for (int k = 0; k < kBK / 16; ++k) {
-              umma_f16_pair(tmem_base + b * kTile, operand_desc<A_MN>(sa + k * k_step_bytes<A_MN>()),
-                            operand_desc<B_MN>(sb + k * k_step_bytes<B_MN>()), a.idesc, accumulate);
-              accumulate = 1;
+              for (int k = 0; k < kBK / 16; ++k)
+                umma_f16_pair(tmem0 + b * kTile, da + (uint64_t)(k * k_step_bytes<A_MN>() >> 4),
+                              db + (uint64_t)(k * k_step_bytes<B_MN>() >> 4), a.idesc, k > 0 || i > 0);
+              umma_commit_pair(&empty[s]);
+              if (i == steps - 1) umma_commit_pair(&acc_full[b]);
             }
-            umma_commit_pair(&empty[s]);
+            __syncwarp();
+            if (++s == kStages) {
+              s = 0;
+              phase ^= 1;
+            }
           }
-          if (!ok) break;
-          umma_commit_pair(&acc_full[b]);
         }
       }
     }
@@ -237,6 +304,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     // ------------------------------------------------ drain + epilogue
     const int q = warp & 3, half = warp >> 2;  // tensor-memory lane quarter; which 128 of the 256 columns
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
+    const Out out{smem + kOutOffset + warp * kOutBytes, lane};
     uint32_t chunk = 0;
     bool ok = true;
     for (int64_t u = pair; u < units.units && ok; u += num_pairs) {
@@ -265,8 +333,9 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         }
       }
       if (!ok) break;
-      epi(acc, tm * kTile + (int64_t)rank * kHalf + q * 32 + lane, tn * kTile + half * 128, split);
+      epi(acc, (int)(tm * kTile) + (int)rank * kHalf + q * 32 + lane, (int)(tn * kTile) + half * 128, split, &tmC, out);
     }
+    if (lane == 0) tma_store_wait_all();
   }
 
   tc_fence_before();
@@ -285,9 +354,12 @@ struct Operand {
   int64_t cols, rows, ld, planes, plane_stride;
 };
 int make_map(CUtensorMap* tm, const Operand& o, bool bf16, bool mn_major);
+// An output [planes][rows][cols] of 2- or 4-byte elements, written in boxes of 32 rows x 128 bytes.
+int make_out_map(CUtensorMap* tm, const Operand& o, int bytes);
 
 template <bool A_MN, bool B_MN, class Epi>
-int launch(const Operand& A, const Operand& B, bool bf16, Args args, const Epi& epi, int device, int sms, cudaStream_t s) {
+int launch(const Operand& A, const Operand& B, bool bf16, Args args, const CUtensorMap& tc, const Epi& epi, int device, int sms,
+           cudaStream_t s) {
   CUtensorMap ta, tb;
   int st = make_map(&ta, A, bf16, A_MN);
   if (st == TCB200_OK) st = make_map(&tb, B, bf16, B_MN);
@@ -303,7 +375,7 @@ int launch(const Operand& A, const Operand& B, bool bf16, Args args, const Epi& 
   const unsigned pairs = (unsigned)std::min<int64_t>(units, std::max(1, sms / 2));
   static std::atomic<uint64_t> configured{0};
   TCB200_CUDA_TRY(ensure_dynamic_smem(pair_gemm_kernel<A_MN, B_MN, Epi>, kSmemBytes, device, configured));
-  TCB200_CUDA_TRY(launch_pdl(pair_gemm_kernel<A_MN, B_MN, Epi>, dim3(2 * pairs), dim3(kThreads), kSmemBytes, s, ta, tb, args, epi));
+  TCB200_CUDA_TRY(launch_pdl(pair_gemm_kernel<A_MN, B_MN, Epi>, dim3(2 * pairs), dim3(kThreads), kSmemBytes, s, ta, tb, tc, args, epi));
   return TCB200_OK;
 }
 
