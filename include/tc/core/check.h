@@ -27,6 +27,10 @@ class Checker {
   bool ok_;
   std::stringstream msg_;
 };
+// Turns a streamed-into Checker into void, so that a check that holds builds neither message nor stream.
+struct Voidify {
+  void operator&(const Checker&) const {}
+};
 template <typename A, typename B>
 std::string describe(const char* op, const A& a, const B& b) {
   std::stringstream ss;
@@ -36,9 +40,12 @@ std::string describe(const char* op, const A& a, const B& b) {
 }  // namespace detail
 }  // namespace tc
 
-#define TC_CHECK(cond) ::tc::detail::Checker(static_cast<bool>(cond), __FILE__, __LINE__, #cond)
+#define TC_CHECK(cond)             \
+  static_cast<bool>(cond) ? (void)0 \
+                          : ::tc::detail::Voidify() & ::tc::detail::Checker(false, __FILE__, __LINE__, #cond)
 #define TC_CHECK_OP_(op, a, b) \
-  ::tc::detail::Checker(((a)op(b)), __FILE__, __LINE__, ::tc::detail::describe(#op, (a), (b)))
+  ((a)op(b)) ? (void)0         \
+             : ::tc::detail::Voidify() & ::tc::detail::Checker(false, __FILE__, __LINE__, ::tc::detail::describe(#op, (a), (b)))
 #define TC_CHECK_EQ(a, b) TC_CHECK_OP_(==, a, b)
 #define TC_CHECK_NE(a, b) TC_CHECK_OP_(!=, a, b)
 #define TC_CHECK_LT(a, b) TC_CHECK_OP_(<, a, b)

@@ -21,5 +21,6 @@ def __getattr__(name):
         return getattr(api, name)
     if name in ("linear_cross_entropy", "topk_distillation"):
         import importlib
-        return getattr(importlib.import_module(".losses", __name__), name)
+        globals()[name] = getattr(importlib.import_module(".losses", __name__), name)  # looked up once
+        return globals()[name]
     raise AttributeError(name)

@@ -1,6 +1,7 @@
 // pybind11 module over the ATen-facing C++ API (the reference's tensor_comprehensions/pybinds/tclib.cc).
 // Everything here goes through tc::aten::compile / run / profile / ATenAutotuner::tune; the extra
 // introspection helpers (sexpr, analyze, match) exist for the CPU-side tests.
+#include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
 #include <sstream>
@@ -88,6 +89,49 @@ struct OnDeviceOf {
     if (!inputs.empty() && inputs[0].is_cuda()) guard.reset(new tc::WithCudaDevice((size_t)inputs[0].get_device()));
   }
   std::unique_ptr<tc::WithCudaDevice> guard;
+};
+
+// ---- losses of a large-vocabulary head (tc/aten/aten_losses.h) as autograd functions ----
+// They run on the current stream of the tensors' device.
+tcb200_stream_t streamOf(const at::Tensor& t) {
+  return t.is_cuda() ? reinterpret_cast<tcb200_stream_t>(c10::cuda::getCurrentCUDAStream(t.get_device()).stream()) : nullptr;
+}
+
+struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& X, const at::Tensor& W,
+                            const at::Tensor& target, int64_t ignoreIndex) {
+    auto r = tc::aten::linearCrossEntropy(X, W, target, ignoreIndex, streamOf(X));
+    ctx->saved_data["ignore_index"] = ignoreIndex;
+    ctx->save_for_backward({X, W, target, r[1]});
+    return r[0];
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    TC_CHECK(!at::GradMode::is_enabled()) << "linear_cross_entropy has no second derivative";
+    if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    auto r = tc::aten::linearCrossEntropyBackward(saved[0], saved[1], saved[2], saved[3], grads[0],
+                                                  ctx->saved_data["ignore_index"].toInt(), ctx->needs_input_grad(0),
+                                                  ctx->needs_input_grad(1), streamOf(saved[0]));
+    return {r[0], r[1], at::Tensor(), at::Tensor()};
+  }
+};
+
+struct TopkDistillation : torch::autograd::Function<TopkDistillation> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& indices,
+                            const at::Tensor& teacher, double temperature) {
+    auto r = tc::aten::topkDistillation(logits, indices, teacher, temperature, streamOf(logits));
+    ctx->saved_data["temperature"] = temperature;
+    ctx->save_for_backward({logits, indices, teacher, r[1]});
+    return r[0];
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    TC_CHECK(!at::GradMode::is_enabled()) << "topk_distillation has no second derivative";
+    if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    return {tc::aten::topkDistillationBackward(saved[0], saved[1], saved[2], saved[3], grads[0],
+                                               ctx->saved_data["temperature"].toDouble(), streamOf(saved[0])),
+            at::Tensor(), at::Tensor(), at::Tensor()};
+  }
 };
 
 }  // namespace
@@ -356,26 +400,20 @@ PYBIND11_MODULE(tclib, m) {
           return r;
         });
 
-  // ---- losses of a large-vocabulary head (tc/aten/aten_losses.h); `stream`: the caller's current one ----
-  auto toStream = [](uintptr_t s) { return reinterpret_cast<tcb200_stream_t>(s); };
+  // ---- losses of a large-vocabulary head: losses.py documents them ----
   m.def("linear_cross_entropy",
-        [toStream](const at::Tensor& x, const at::Tensor& w, const at::Tensor& target, int64_t ignoreIndex, uintptr_t stream) {
-          return tc::aten::linearCrossEntropy(x, w, target, ignoreIndex, toStream(stream));
-        });
-  m.def("linear_cross_entropy_backward",
-        [toStream](const at::Tensor& x, const at::Tensor& w, const at::Tensor& target, const at::Tensor& lse,
-                   const at::Tensor& grad, int64_t ignoreIndex, bool needX, bool needW, uintptr_t stream) {
-          return tc::aten::linearCrossEntropyBackward(x, w, target, lse, grad, ignoreIndex, needX, needW, toStream(stream));
+        [](const at::Tensor& X, const at::Tensor& W, const at::Tensor& target, int64_t ignoreIndex) {
+          if (at::GradMode::is_enabled() && (X.requires_grad() || W.requires_grad()))
+            return LinearCrossEntropy::apply(X, W, target, ignoreIndex);
+          return tc::aten::linearCrossEntropy(X, W, target, ignoreIndex, streamOf(X))[0];
         });
   m.def("topk_distillation",
-        [toStream](const at::Tensor& logits, const at::Tensor& indices, const at::Tensor& teacher, double temperature,
-                   uintptr_t stream) {
-          return tc::aten::topkDistillation(logits, indices, teacher, temperature, toStream(stream));
-        });
-  m.def("topk_distillation_backward",
-        [toStream](const at::Tensor& logits, const at::Tensor& indices, const at::Tensor& teacher, const at::Tensor& stats,
-                   const at::Tensor& grad, double temperature, uintptr_t stream) {
-          return tc::aten::topkDistillationBackward(logits, indices, teacher, stats, grad, temperature, toStream(stream));
+        [](const at::Tensor& logits, const at::Tensor& indices, const at::Tensor& teacher, double temperature) {
+          TC_CHECK(!(at::GradMode::is_enabled() && teacher.requires_grad()))
+              << "topk_distillation gives the teacher no gradient: pass teacher.detach()";
+          if (at::GradMode::is_enabled() && logits.requires_grad())
+            return TopkDistillation::apply(logits, indices, teacher, temperature);
+          return tc::aten::topkDistillation(logits, indices, teacher, temperature, streamOf(logits))[0];
         });
 
   m.def("set_flag", [](const std::string& name, const std::string& value) {

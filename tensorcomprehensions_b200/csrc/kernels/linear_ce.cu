@@ -89,69 +89,11 @@ struct Head {
 // ---- rows -----------------------------------------------------------------------------------------------------------
 struct Rows {
   Head* head;
-  int* source;    // [n_pad] live row -> row
   int* place;     // [n] row -> live row, -1 without a target
   int* target;    // [n_pad] of a live row; -1: outside [0, V)
   float* share;   // [n_pad] g of a live row / gscale (backward)
   float* lse;     // [n_pad] of a live row (backward)
 };
-
-// One block walks over the rows in order: the order of the live rows, and with it every later sum, does not depend on timing.
-template <typename Index>
-__global__ void __launch_bounds__(1024) rows_kernel(const Index* target, int64_t n, int64_t v, int64_t ignore,
-                                                    const float* g, int64_t g_stride, const float* lse, Rows r) {
-  __shared__ int warp_count[32];
-  __shared__ float warp_max[32];
-  pdl_sync();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int base = 0;
-  float top = 0.f;
-  for (int64_t i0 = 0; i0 < n; i0 += 1024) {
-    const int64_t i = i0 + threadIdx.x;
-    const int64_t t = i < n ? (int64_t)target[i] : ignore;
-    const bool live = i < n && t != ignore;
-    const unsigned votes = __ballot_sync(0xffffffffu, live);
-    if (lane == 0) warp_count[warp] = __popc(votes);
-    __syncthreads();
-    int before = base, all = 0;
-    for (int w = 0; w < 32; ++w) {
-      if (w < warp) before += warp_count[w];
-      all += warp_count[w];
-    }
-    const int at = before + __popc(votes & ((1u << lane) - 1));
-    if (live) {
-      r.source[at] = (int)i;
-      r.target[at] = t >= 0 && t < v ? (int)t : -1;
-      if (g) {
-        const float x = g[i * g_stride];
-        r.share[at] = x;
-        r.lse[at] = lse[i];
-        const float ax = fabsf(x);
-        if (ax <= 3.402823466e38f) top = fmaxf(top, ax);  // the largest finite one: not NaN, not infinite
-      }
-    }
-    if (i < n) r.place[i] = live ? at : -1;
-    base += all;
-    __syncthreads();
-  }
-  if (g) {
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) warp_max[warp] = top;
-    __syncthreads();
-    for (int w = 0; w < 32; ++w) top = fmaxf(top, warp_max[w]);
-    // dZ is kept with g / max|g|: where all rows share one g, as under a mean, that is exactly 1 and the rounding
-    // of dZ to 16 bits does not meet g's significand
-    for (int i = threadIdx.x; i < base; i += 1024) {
-      const float x = r.share[i];
-      r.share[i] = r.target[i] < 0 ? __int_as_float(0x7fffffff) : (top > 0.f ? x / top : x);
-    }
-  }
-  if (threadIdx.x == 0) {
-    r.head->live = base;
-    r.head->status = 0;
-    r.head->gscale = top > 0.f ? top : 1.f;
-  }
-}
 
 // ---- operands -------------------------------------------------------------------------------------------------------
 template <typename T>
@@ -175,47 +117,139 @@ __device__ __forceinline__ void split3(float v, uint16_t* p) {
   p[2] = bits(__float2bfloat16_rn(r));
 }
 
-// Rows of X or W as operand planes [planes][rows_cap][dp], dp = d rounded up to 8, the padding zero.  `source` picks live
-// rows: those behind the last one, up to a whole tile, are zero.  A thread makes eight columns; the input is read once.
+// Eight columns of a row of X or W as operand planes; what lies behind column d is zero.
+template <typename T>
+__device__ __forceinline__ void pack8(const T* src, int64_t left, uint16_t* dst, int64_t plane) {
+  alignas(16) T v[8];
+  if (left >= 8 && ((uintptr_t)src & 15) == 0) {
+#pragma unroll
+    for (int q = 0; q < (int)sizeof(T) / 2; ++q) reinterpret_cast<uint4*>(v)[q] = __ldg(reinterpret_cast<const uint4*>(src) + q);
+  } else {
+    memset(v, 0, sizeof(v));
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < left) v[j] = src[j];
+  }
+  if (sizeof(T) == 4) {
+    alignas(16) uint16_t w[3][8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint16_t p[3];
+      split3(to_float(v[j]), p);
+      w[0][j] = p[0]; w[1][j] = p[1]; w[2][j] = p[2];
+    }
+#pragma unroll
+    for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4*>(dst + p * plane) = *reinterpret_cast<uint4*>(w[p]);
+  } else {
+    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(v);
+  }
+}
+
+// Entries of W as operand planes [planes][rows][dp], dp = d rounded up to 8.
 template <typename T>
 __global__ void __launch_bounds__(256) pack_kernel(const T* in, int64_t ld, int64_t rows, int64_t d, int64_t dp,
-                                                   const int* source, const int* live, uint16_t* out, int64_t plane) {
+                                                   uint16_t* out, int64_t plane) {
   pdl_sync();
-  const bool f32 = sizeof(T) == 4;
-  const int64_t per_row = dp / 8;
-  const int64_t have = live ? *live : rows;
-  const int64_t total = (live ? (have + kTile - 1) / kTile * kTile : rows) * per_row;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+  // a piece has fewer than 2^31 groups of eight (it is 256 MiB, or 4096 entries of at most 2^20 columns)
+  const uint32_t per_row = (uint32_t)(dp / 8), total = (uint32_t)rows * per_row;
+  for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < total; i += gridDim.x * blockDim.x) {
     const int64_t r = i / per_row, c = (i % per_row) * 8;
-    alignas(16) T v[8];
-    memset(v, 0, sizeof(v));
-    if (r < have) {
-      const T* src = in + (source ? (int64_t)source[r] : r) * ld + c;
-      if (c + 8 <= d && ((uintptr_t)src & 15) == 0) {
-#pragma unroll
-        for (int q = 0; q < (int)sizeof(T) / 2; ++q)
-          reinterpret_cast<uint4*>(v)[q] = __ldg(reinterpret_cast<const uint4*>(src) + q);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (c + j < d) v[j] = src[j];
-      }
-    }
-    uint16_t* dst = out + r * dp + c;
-    if (f32) {
-      alignas(16) uint16_t w[3][8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint16_t p[3];
-        split3(to_float(v[j]), p);
-        w[0][j] = p[0]; w[1][j] = p[1]; w[2][j] = p[2];
-      }
-#pragma unroll
-      for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4*>(dst + p * plane) = *reinterpret_cast<uint4*>(w[p]);
-    } else {
-      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(v);
+    pack8(in + r * ld + c, d - c, out + r * dp + c, plane);
+  }
+}
+
+// The rows with a target, and X of them as operand planes [planes][n_pad][dp]; rows behind the last live one, up to a whole
+// tile, are zero.  Every block reads all targets (and all g, for the largest of them) and knows from them where its own
+// rows go: one launch instead of two that wait for one another, and the order of the live rows, and with it every later
+// sum, does not depend on timing.
+constexpr int kRowThreads = 512;
+template <typename T, typename Index>
+__global__ void __launch_bounds__(kRowThreads) rows_kernel(const Index* target, int64_t n, int64_t v, int64_t ignore,
+                                                           const float* g, int64_t g_stride, const float* lse, Rows r,
+                                                           const T* x, int64_t ld, int64_t d, int64_t dp, uint16_t* out,
+                                                           int64_t plane) {
+  __shared__ int before_of[kRowThreads / 32], all_of[kRowThreads / 32];
+  __shared__ float top_of[kRowThreads / 32];
+  __shared__ int list[kRowThreads];
+  pdl_sync();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t per_block = (n + gridDim.x - 1) / gridDim.x;
+  const int64_t r0 = min(n, blockIdx.x * per_block), r1 = min(n, r0 + per_block);
+  int before = 0, all = 0;
+  float top = 0.f;
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < n; i += kRowThreads) {
+    const bool live = (int64_t)target[i] != ignore;
+    all += live;
+    before += live && i < r0;
+    if (g && live) {
+      const float ax = fabsf(g[i * g_stride]);
+      if (ax <= 3.402823466e38f) top = fmaxf(top, ax);  // the largest finite one: not NaN, not infinite
     }
   }
+  for (int o = 16; o; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  if (lane == 0) {
+    before_of[warp] = before;
+    all_of[warp] = all;
+    top_of[warp] = top;
+  }
+  __syncthreads();
+  before = all = 0;
+  for (int w = 0; w < kRowThreads / 32; ++w) {
+    before += before_of[w];
+    all += all_of[w];
+    top = fmaxf(top, top_of[w]);
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    r.head->live = all;
+    r.head->status = 0;
+    r.head->gscale = top > 0.f ? top : 1.f;
+  }
+  const uint32_t per_row = (uint32_t)(dp / 8);
+  // 512 rows at a time: their places, then their X
+  for (int64_t base = r0; base < r1; base += kRowThreads) {
+    const int64_t i = base + threadIdx.x;
+    const int64_t t = i < r1 ? (int64_t)target[i] : ignore;
+    const bool live = t != ignore;
+    const unsigned votes = __ballot_sync(0xffffffffu, live);
+    __syncthreads();  // the counts and the list of the round before have been read
+    if (lane == 0) before_of[warp] = __popc(votes);
+    __syncthreads();
+    int at = __popc(votes & ((1u << lane) - 1)), count = 0;
+    for (int w = 0; w < kRowThreads / 32; ++w) {
+      if (w < warp) at += before_of[w];
+      count += before_of[w];
+    }
+    if (i < r1) r.place[i] = live ? before + at : -1;
+    if (live) {
+      const bool inside = t >= 0 && t < v;
+      list[at] = (int)(i - base);
+      r.target[before + at] = inside ? (int)t : -1;
+      if (g) {
+        // dZ is kept with g / max|g|: where all rows share one g, as under a mean, that is exactly 1 and the rounding
+        // of dZ to 16 bits does not meet g's significand
+        const float x = g[i * g_stride];
+        r.share[before + at] = !inside ? __int_as_float(0x7fffffff) : top > 0.f ? x / top : x;
+        r.lse[before + at] = lse[i];
+      }
+    }
+    __syncthreads();
+    for (uint32_t k = threadIdx.x; k < (uint32_t)count * per_row; k += kRowThreads) {
+      const uint32_t j = k / per_row;
+      const int64_t c = (k % per_row) * 8;
+      pack8(x + (base + list[j]) * ld + c, d - c, out + (before + j) * dp + c, plane);
+    }
+    before += count;
+  }
+  const int64_t end = (all + (int64_t)kTile - 1) / kTile * kTile;
+  for (int64_t k = blockIdx.x * (int64_t)kRowThreads + threadIdx.x; k < (end - all) * per_row; k += (int64_t)gridDim.x * kRowThreads)
+#pragma unroll
+    for (int p = 0; p < (sizeof(T) == 4 ? 3 : 1); ++p)
+      *reinterpret_cast<uint4*>(out + p * plane + all * dp + k * 8) = make_uint4(0, 0, 0, 0);
 }
 
 // ---- epilogues ------------------------------------------------------------------------------------------------------
@@ -253,43 +287,55 @@ struct ForwardEpi {
   }
 };
 
-// Joins the parts of a row: lse, and the loss lse - z_target.  32 rows x 8 parts a block; a row's parts are added in a
-// fixed order.
-__global__ void __launch_bounds__(256) join_kernel(Rows r, const float2* part, const float* hit, int64_t parts,
-                                                   int64_t n_pad, int64_t n, float* loss, float* lse, int* dev_status) {
-  pdl_sync();
-  if (dev_status && r.head->status && blockIdx.x == 0 && threadIdx.x + threadIdx.y == 0)
-    atomicCAS(dev_status, 0, r.head->status);
-  __shared__ float2 share[8][33];
-  const int64_t i = blockIdx.x * 32 + threadIdx.x;
-  const int64_t at = i < n ? r.place[i] : -1;
+// Joins the parts of a row: lse, and the loss lse - z_target.  32 rows x 32 lanes of parts a block, four loads in flight a
+// thread; a row's parts are joined in a fixed order.
+struct Running {
   float top = -INFINITY, sum = 0.f;
-  if (at >= 0) {
-    for (int64_t p = threadIdx.y; p < parts; p += 8) {
-      const float2 x = part[p * n_pad + at];
-      // fmaxf drops a NaN maximum; its sum is NaN then too and survives
-      const float m = fmaxf(top, x.x), shift = m == -INFINITY ? 0.f : m;
-      sum = sum * exp_neg(top - shift) + x.y * exp_neg(x.x - shift);
-      top = m;
-    }
-  }
-  share[threadIdx.y][threadIdx.x] = make_float2(top, sum);
-  __syncthreads();
-  if (threadIdx.y != 0 || i >= n) return;
-  for (int k = 1; k < 8; ++k) {
-    const float2 x = share[k][threadIdx.x];
+  __device__ __forceinline__ void join(float2 x) {
+    // fmaxf drops a NaN maximum; its sum is NaN then too and survives
     const float m = fmaxf(top, x.x), shift = m == -INFINITY ? 0.f : m;
     sum = sum * exp_neg(top - shift) + x.y * exp_neg(x.x - shift);
     top = m;
   }
+};
+__global__ void __launch_bounds__(1024) join_kernel(Rows r, const float2* part, const float* hit, int64_t parts,
+                                                    int64_t n_pad, int64_t n, float* loss, float* lse, int* dev_status) {
+  __shared__ float2 share[32][33];
+  pdl_sync();
+  if (dev_status && r.head->status && blockIdx.x == 0 && threadIdx.x + threadIdx.y == 0)
+    atomicCAS(dev_status, 0, r.head->status);
+  const int64_t i = blockIdx.x * 32 + threadIdx.x;
+  const int64_t at = i < n ? r.place[i] : -1;
+  const float2 none = make_float2(-INFINITY, 0.f);
+  Running run;
+  if (at >= 0) {
+    for (int64_t p = threadIdx.y; p < parts; p += 128) {
+      float2 x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = p + 32 * k < parts ? part[(p + 32 * k) * n_pad + at] : none;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) run.join(x[k]);
+    }
+  }
+  share[threadIdx.y][threadIdx.x] = make_float2(run.top, run.sum);
+  __syncthreads();
+  // row threadIdx.y of the block, its 32 lanes joined by a warp
+  const float2 mine = share[threadIdx.x][threadIdx.y];
+  run.top = mine.x;
+  run.sum = mine.y;
+  for (int o = 16; o; o >>= 1)
+    run.join(make_float2(__shfl_xor_sync(0xffffffffu, run.top, o), __shfl_xor_sync(0xffffffffu, run.sum, o)));
+  const int64_t row = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x != 0 || row >= n) return;
+  const int place = r.place[row];
   const float nan = __int_as_float(0x7fffffff);
-  float l = top + logf(sum), e = 0.f;
-  if (at < 0) l = 0.f;
-  else if (r.target[at] < 0) e = nan;  // a target outside the vocabulary
-  else e = (top - hit[at]) + logf(sum);
-  if (r.head->status) l = e = nan;     // a wait gave up: no number is better than a wrong one
-  loss[i] = e;
-  lse[i] = l;
+  float l = run.top + logf(run.sum), e = 0.f;
+  if (place < 0) l = 0.f;
+  else if (r.target[place] < 0) e = nan;  // a target outside the vocabulary
+  else e = (run.top - hit[place]) + logf(run.sum);
+  if (r.head->status) l = e = nan;        // a wait gave up: no number is better than a wrong one
+  loss[row] = e;
+  lse[row] = l;
 }
 
 // dZ of a piece, as operand planes [planes][n_pad][ld].  f16 values carry 2^14: probabilities from 2^-28 up then keep all
@@ -460,7 +506,7 @@ struct Layout {
   int splits;
   int64_t fwd_bytes, bwd_bytes;
   // byte offsets
-  int64_t source, place, target, share, lse, hit, part, x, w_fwd, w_bwd, dz, sums;
+  int64_t place, target, share, lse, hit, part, x, w_fwd, w_bwd, dz, sums;
 };
 
 bool pack_w(const tcb200_linear_ce_t& p) { return p.dtype == TCB200_F32 || p.pack_w; }
@@ -508,7 +554,6 @@ int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
     return here;
   };
   take(sizeof(Head));
-  l->source = take(l->n_pad * 4);
   l->place = take(p.N * 4);
   l->target = take(l->n_pad * 4);
   l->share = take(l->n_pad * 4);
@@ -530,7 +575,6 @@ int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
 Rows rows_of(char* ws, const Layout& l) {
   Rows r;
   r.head = reinterpret_cast<Head*>(ws);
-  r.source = reinterpret_cast<int*>(ws + l.source);
   r.place = reinterpret_cast<int*>(ws + l.place);
   r.target = reinterpret_cast<int*>(ws + l.target);
   r.share = reinterpret_cast<float*>(ws + l.share);
@@ -538,28 +582,33 @@ Rows rows_of(char* ws, const Layout& l) {
   return r;
 }
 
-int launch_rows(const tcb200_linear_ce_t& p, const void* target, const float* g, int64_t g_stride, const float* lse,
-                const Rows& r, cudaStream_t s) {
-  if (p.index_bytes == 8)
-    TCB200_CUDA_TRY(launch_pdl(rows_kernel<int64_t>, dim3(1), dim3(1024), 0, s, static_cast<const int64_t*>(target), p.N,
-                               p.V, p.ignore_index, g, g_stride, lse, r));
-  else
-    TCB200_CUDA_TRY(launch_pdl(rows_kernel<int32_t>, dim3(1), dim3(1024), 0, s, static_cast<const int32_t*>(target), p.N,
-                               p.V, p.ignore_index, g, g_stride, lse, r));
+template <typename T, typename Index>
+int launch_rows_typed(const tcb200_linear_ce_t& p, const Layout& l, const void* X, const void* target, const float* g,
+                      int64_t g_stride, const float* lse, const Rows& r, void* out, int sms, cudaStream_t s) {
+  // blocks enough for the rows' copies, zero rows of the last tile among them
+  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(l.n_pad * (l.dp / 8), kRowThreads), 2ll * sms);
+  TCB200_CUDA_TRY(launch_pdl(rows_kernel<T, Index>, dim3(blocks), dim3(kRowThreads), 0, s, static_cast<const Index*>(target),
+                             p.N, p.V, p.ignore_index, g, g_stride, lse, r, static_cast<const T*>(X), p.ldx, p.D, l.dp,
+                             static_cast<uint16_t*>(out), l.n_pad * l.dp));
   return TCB200_OK;
 }
+// f16 and bf16 are copied as they are
+int launch_rows(const tcb200_linear_ce_t& p, const Layout& l, const void* X, const void* target, const float* g,
+                int64_t g_stride, const float* lse, const Rows& r, void* out, int sms, cudaStream_t s) {
+  const bool f32 = p.dtype == TCB200_F32, wide = p.index_bytes == 8;
+  auto fn = f32 ? (wide ? launch_rows_typed<float, int64_t> : launch_rows_typed<float, int32_t>)
+                : (wide ? launch_rows_typed<__half, int64_t> : launch_rows_typed<__half, int32_t>);
+  return fn(p, l, X, target, g, g_stride, lse, r, out, sms, s);
+}
 
-int launch_pack(const tcb200_linear_ce_t& p, const Layout& l, const void* in, int64_t ld, int64_t rows, const int* source,
-                const int* live, void* out, int64_t plane, int sms, cudaStream_t s) {
-  const int64_t items = (live ? l.n_pad : rows) * (l.dp / 8);
-  const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(items, 256), 8ll * sms)));
+int launch_pack(const tcb200_linear_ce_t& p, const Layout& l, const void* in, int64_t rows, void* out, int64_t plane, int sms,
+                cudaStream_t s) {
+  const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows * (l.dp / 8), 256), 8ll * sms)));
   uint16_t* o = static_cast<uint16_t*>(out);
-  cudaError_t e;
   if (p.dtype == TCB200_F32)
-    e = launch_pdl(pack_kernel<float>, grid, dim3(256), 0, s, static_cast<const float*>(in), ld, rows, p.D, l.dp, source, live, o, plane);
-  else  // f16 and bf16 are copied as they are
-    e = launch_pdl(pack_kernel<__half>, grid, dim3(256), 0, s, static_cast<const __half*>(in), ld, rows, p.D, l.dp, source, live, o, plane);
-  TCB200_CUDA_TRY(e);
+    TCB200_CUDA_TRY(launch_pdl(pack_kernel<float>, grid, dim3(256), 0, s, static_cast<const float*>(in), p.ldw, rows, p.D, l.dp, o, plane));
+  else
+    TCB200_CUDA_TRY(launch_pdl(pack_kernel<__half>, grid, dim3(256), 0, s, static_cast<const __half*>(in), p.ldw, rows, p.D, l.dp, o, plane));
   return TCB200_OK;
 }
 
@@ -593,7 +642,7 @@ int w_operand(const tcb200_linear_ce_t& p, const Layout& l, const void* W, int64
     return TCB200_OK;
   }
   *o = {packed, l.dp, v, l.dp, l.planes, piece * l.dp};
-  return launch_pack(p, l, base, p.ldw, v, nullptr, nullptr, packed, piece * l.dp, sms, s);
+  return launch_pack(p, l, base, v, packed, piece * l.dp, sms, s);
 }
 
 int current_device(int* device) {
@@ -677,8 +726,7 @@ int tcb200_linear_ce_forward(const tcb200_linear_ce_t* problem, const void* X, c
   char* ws = static_cast<char*>(workspace);
   const Rows r = rows_of(ws, l);
   int* status = &r.head->status;
-  if ((st = launch_rows(p, target, nullptr, 0, nullptr, r, s)) != TCB200_OK) return st;
-  st = launch_pack(p, l, X, p.ldx, p.N, r.source, &r.head->live, ws + l.x, l.n_pad * l.dp, sms, s);
+  st = launch_rows(p, l, X, target, nullptr, 0, nullptr, r, ws + l.x, sms, s);
   if (st != TCB200_OK) return st;
   const pg::Operand x{ws + l.x, l.dp, l.n_pad, l.dp, l.planes, l.n_pad * l.dp};
   float2* part = reinterpret_cast<float2*>(ws + l.part);
@@ -692,7 +740,7 @@ int tcb200_linear_ce_forward(const tcb200_linear_ce_t* problem, const void* X, c
                                   CUtensorMap{}, e, device, sms, s);
     if (st != TCB200_OK) return st;
   }
-  TCB200_CUDA_TRY(launch_pdl(join_kernel, dim3((unsigned)ceil_div(p.N, 32)), dim3(32, 8), 0, s, r,
+  TCB200_CUDA_TRY(launch_pdl(join_kernel, dim3((unsigned)ceil_div(p.N, 32)), dim3(32, 32), 0, s, r,
                              static_cast<const float2*>(part), static_cast<const float*>(hit), l.parts, l.n_pad, p.N, loss, lse, dev_status));
   return TCB200_OK;
 }
@@ -719,8 +767,7 @@ int tcb200_linear_ce_backward(const tcb200_linear_ce_t* problem, const void* X, 
   char* ws = static_cast<char*>(workspace);
   const Rows r = rows_of(ws, l);
   int* status = &r.head->status;
-  if ((st = launch_rows(p, target, grad_loss, grad_stride, lse, r, s)) != TCB200_OK) return st;
-  st = launch_pack(p, l, X, p.ldx, p.N, r.source, &r.head->live, ws + l.x, l.n_pad * l.dp, sms, s);
+  st = launch_rows(p, l, X, target, grad_loss, grad_stride, lse, r, ws + l.x, sms, s);
   if (st != TCB200_OK) return st;
   switch (p.dtype) {
     case TCB200_F32:

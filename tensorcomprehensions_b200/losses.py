@@ -7,33 +7,9 @@
     loss = tc.topk_distillation(logits, indices, teacher, temperature=2.0)
 
 Both run on tensors of one CUDA device, on its current stream, without synchronising; they may be captured into CUDA graphs.
-There is no CPU or eager fallback.  The reference's operator library has no loss (its tc/library ends at the layers).
+There is no CPU or eager fallback, and no second derivative.  The reference's operator library has no loss (its tc/library ends at the layers).
 """
-import torch
-from torch.autograd.function import once_differentiable
-
 from . import tclib
-
-
-def _stream(t):
-    return torch.cuda.current_stream(t.device).cuda_stream if t.is_cuda else 0
-
-
-class _LinearCrossEntropy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, X, W, target, ignore_index):
-        loss, lse = tclib.linear_cross_entropy(X, W, target, ignore_index, _stream(X))
-        ctx.ignore_index = ignore_index
-        ctx.save_for_backward(X, W, target, lse)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        X, W, target, lse = ctx.saved_tensors
-        dX, dW = tclib.linear_cross_entropy_backward(X, W, target, lse, grad, ctx.ignore_index, ctx.needs_input_grad[0],
-                                                     ctx.needs_input_grad[1], _stream(X))
-        return dX, dW, None, None
 
 
 def linear_cross_entropy(X, W, target, ignore_index=-100):
@@ -47,25 +23,7 @@ def linear_cross_entropy(X, W, target, ignore_index=-100):
     X and W have their type, are summed in float32 and rounded once (between the two products the gradient of z is rounded
     to the inputs' 16-bit type; float32 inputs keep float32 accuracy throughout).  A wrong type, size, stride or device
     raises RuntimeError."""
-    return _LinearCrossEntropy.apply(X, W, target, int(ignore_index))
-
-
-class _TopkDistillation(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, indices, teacher, temperature):
-        loss, stats = tclib.topk_distillation(logits, indices, teacher, temperature, _stream(logits))
-        ctx.temperature = temperature
-        ctx.save_for_backward(logits, indices, teacher, stats)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        logits, indices, teacher, stats = ctx.saved_tensors
-        d = None
-        if ctx.needs_input_grad[0]:
-            d = tclib.topk_distillation_backward(logits, indices, teacher, stats, grad, ctx.temperature, _stream(logits))
-        return d, None, None, None
+    return tclib.linear_cross_entropy(X, W, target, ignore_index)
 
 
 def topk_distillation(logits, indices, teacher, temperature=1.0):
@@ -79,6 +37,4 @@ def topk_distillation(logits, indices, teacher, temperature=1.0):
     loss 0 and gradient 0; an index of V or more makes the row's loss and gradient NaN; an index that stands twice counts
     twice.  The gradient is that of the logits, in their type; the teacher gets none.  A wrong type, size, stride,
     device or temperature raises RuntimeError."""
-    if teacher.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("topk_distillation gives the teacher no gradient: pass teacher.detach()")
-    return _TopkDistillation.apply(logits, indices, teacher, float(temperature))
+    return tclib.topk_distillation(logits, indices, teacher, temperature)
