@@ -7,8 +7,7 @@
 //
 // Forward: a cluster of CTAs takes a row (one CTA where the rows alone fill the device, up to eight where there are few), each
 // thread keeps the running maximum and sum of its elements, the CTAs' pairs meet in the first CTA's shared memory.  The
-// K entries and the student's logits at their places are fetched before the pass over the row, so their latency hides
-// behind it.
+// K entries are fetched before the pass over the row, so their latency hides behind it.
 // Backward: the row's maximum and sum are known, so a CTA takes any stretch of a row: it writes T g p for all of it, then, behind a block barrier,
 // writes the entries' places again with q taken off.  p - q is formed in fp32 and rounded once.
 #include <cuda_bf16.h>
@@ -21,7 +20,7 @@
 namespace tcb200 {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T> __device__ __forceinline__ float load1(const T* p);
@@ -44,9 +43,23 @@ __device__ __forceinline__ uint4 load_raw(const void* p) {
 __device__ __forceinline__ void store_raw(void* p, const uint4& v) {
   asm volatile("st.global.cs.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
+// base-2 exponential; results below the smallest normal number become 0
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Eight 16-bit or four 32-bit elements of 16 bytes.  scaled(x): (x - top) * scale.  float32 subtracts first, which is exact
+// where exp is not small; in 16 bits the product is folded into one multiply-add, whose error (2^-24 of |top| * scale) is far
+// below the elements' own.
 template <typename T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int n = 4;
+  static constexpr bool exact = true;
+  static __device__ __forceinline__ float maximum(const uint4& r) {
+    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+  }
   static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
     v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
   }
@@ -56,6 +69,12 @@ template <> struct Vec<float> {
 };
 template <> struct Vec<__half> {
   static constexpr int n = 8;
+  static constexpr bool exact = false;
+  static __device__ __forceinline__ float maximum(const uint4& r) {
+    const __half2* h = reinterpret_cast<const __half2*>(&r);
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
   static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -76,6 +95,12 @@ template <> struct Vec<__half> {
 };
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int n = 8;
+  static constexpr bool exact = false;
+  static __device__ __forceinline__ float maximum(const uint4& r) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
   static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -113,48 +138,66 @@ struct Entries {
   }
 };
 
-// Running maximum and sum of exp((x - maximum) * scale).  An empty pair is (-inf, 0).
+template <typename T>
+__device__ __forceinline__ float exp_from(float x, float top, float neg_top_scaled, float scale) {
+  return exp2_fast(Vec<T>::exact ? (x - top) * scale : fmaf(x, scale, neg_top_scaled));
+}
+
+// Running maximum and sum of exp((x - maximum) * scale).  An empty pair is (-inf, 0).  A maximum drops NaN; the sum keeps it.
 struct Running {
   float top = -INFINITY, sum = 0.f;
   __device__ __forceinline__ void join(float t, float s, float scale) {
     const float m = fmaxf(top, t), shift = m == -INFINITY ? 0.f : m;
-    sum = sum * exp2f((top - shift) * scale) + s * exp2f((t - shift) * scale);
+    sum = sum * exp2_fast((top - shift) * scale) + s * exp2_fast((t - shift) * scale);
     top = m;
   }
-  template <int N>
-  __device__ __forceinline__ void add(const float* v, float scale) {
-    float m = v[0];
+  // moves the maximum up to m before elements of at most m are added
+  __device__ __forceinline__ void raise(float m, float scale) {
+    if (m > top) {
+      sum *= exp2_fast((top - m) * scale);  // 0 while top is -inf
+      top = m;
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void one(float x, float scale) {
+    raise(x, scale);
+    const float shift = top == -INFINITY ? 0.f : top;
+    sum += exp_from<T>(x, shift, -shift * scale, scale);
+  }
+  template <typename T, int U>
+  __device__ __forceinline__ void vectors(const uint4 (&raw)[U], float scale) {
+    float m = Vec<T>::maximum(raw[0]);
 #pragma unroll
-    for (int j = 1; j < N; ++j) m = fmaxf(m, v[j]);
-    m = fmaxf(m, top);
-    const float shift = m == -INFINITY ? 0.f : m;
-    float s = 0.f;
+    for (int u = 1; u < U; ++u) m = fmaxf(m, Vec<T>::maximum(raw[u]));
+    raise(m, scale);
+    const float shift = top == -INFINITY ? 0.f : top, neg = -shift * scale;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < N; ++j) s += exp2f((v[j] - shift) * scale);
-    sum = (m > top ? sum * exp2f((top - shift) * scale) : sum) + s;  // sum is 0 while top is -inf
-    top = m;
+    for (int u = 0; u < U; ++u) {
+      float x[Vec<T>::n];
+      Vec<T>::unpack(raw[u], x);
+#pragma unroll
+      for (int j = 0; j < Vec<T>::n; ++j) s[j & 3] += exp_from<T>(x[j], shift, neg, scale);
+    }
+    sum += (s[0] + s[1]) + (s[2] + s[3]);
   }
 };
 
-// All threads get the block's pair; `share` holds one pair a warp.  Pairs are joined in a fixed order.
-__device__ __forceinline__ Running block_join(Running r, float scale, float2* share) {
-  for (int o = 16; o; o >>= 1)
-    r.join(__shfl_xor_sync(0xffffffffu, r.top, o), __shfl_xor_sync(0xffffffffu, r.sum, o), scale);
+// All threads get the block's pairs (two at once, of two scales); `share` holds two pairs a warp.  Pairs are joined in a
+// fixed order.
+__device__ __forceinline__ void block_join(Running& a, float scale_a, Running& b, float scale_b, float4* share) {
+  for (int o = 16; o; o >>= 1) {
+    a.join(__shfl_xor_sync(0xffffffffu, a.top, o), __shfl_xor_sync(0xffffffffu, a.sum, o), scale_a);
+    b.join(__shfl_xor_sync(0xffffffffu, b.top, o), __shfl_xor_sync(0xffffffffu, b.sum, o), scale_b);
+  }
+  if ((threadIdx.x & 31) == 0) share[threadIdx.x >> 5] = make_float4(a.top, a.sum, b.top, b.sum);
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) share[threadIdx.x >> 5] = make_float2(r.top, r.sum);
-  __syncthreads();
-  Running all;
-  for (int w = 0; w < kThreads / 32; ++w) all.join(share[w].x, share[w].y, scale);
-  return all;
-}
-__device__ __forceinline__ float block_sum(float v, float2* share) {
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) share[threadIdx.x >> 5].x = v;
-  __syncthreads();
-  float all = 0.f;
-  for (int w = 0; w < kThreads / 32; ++w) all += share[w].x;
-  return all;
+  a = b = Running();
+  for (int w = 0; w < kThreads / 32; ++w) {
+    const float4 x = share[w];
+    a.join(x.x, x.y, scale_a);
+    b.join(x.z, x.w, scale_b);
+  }
 }
 
 // [first, last) of a row for part `i` of `n`: whole 64-element steps, so that the parts' inner bounds keep the alignment of the row
@@ -169,65 +212,53 @@ constexpr int kMaxCluster = 8;
 template <typename T>
 __global__ void __launch_bounds__(kThreads) distill_forward_kernel(const T* logits, int64_t ld, int64_t v, Entries e,
                                                                    float temperature, float* loss, float* stats, int parts) {
-  extern __shared__ float entry_mem[];       // teacher / T, then the student's logit of each entry
-  __shared__ float2 share[kThreads / 32];
+  __shared__ float4 share[kThreads / 32];
+  __shared__ float sums[kThreads / 32];
   __shared__ float2 gathered[kMaxCluster];
-  __shared__ int bad;
   pdl_sync();
   const int rank = (int)(blockIdx.x % parts);
   const int64_t row = blockIdx.x / parts;
   const T* z = logits + row * ld;
-  float* et = entry_mem;
-  float* ez = entry_mem + e.k;
   const float inv = 1.f / temperature, scale = kLog2e * inv;
-  if (threadIdx.x == 0) bad = 0;
-  __syncthreads();
-  if (rank == 0) {
-    for (int j = threadIdx.x; j < e.k; j += kThreads) {
-      const int64_t i = e.index(row, j);
-      float t = e.logit(row, j), s = 0.f;
-      if (i >= v) bad = 1;
-      if (i < 0) t = -INFINITY;
-      if (i >= 0 && i < v) s = load1(z + i);
-      et[j] = t;
-      ez[j] = s;
-    }
-  }
+  // The first entry of a thread (all of them where K is at most the block) is fetched here and used behind the row.
+  const bool mine = rank == 0 && threadIdx.x < e.k;
+  const int64_t place = mine ? e.index(row, threadIdx.x) : -1;
+  const float teacher = mine ? e.logit(row, threadIdx.x) : 0.f;
   int64_t first, last;
   stretch(v, rank, parts, &first, &last);
   Running r;
   constexpr int W = Vec<T>::n;
   // elements up to the first 16-byte boundary, whole vectors, the rest
   const int64_t head = min(last, first + (int64_t)((16 - ((uintptr_t)(z + first) & 15)) & 15) / (int64_t)sizeof(T));
-  const int64_t vecs = (last - head) / W;
-  if (first + threadIdx.x < head) {
-    const float x = load1(z + first + threadIdx.x);
-    r.add<1>(&x, scale);
-  }
+  const int vecs = (int)((last - head) / W);
   const T* body = z + head;
-  int64_t i = threadIdx.x;
+  int i = threadIdx.x;
   constexpr int U = 4;  // loads in flight a thread
   for (; i + (U - 1) * kThreads < vecs; i += U * kThreads) {
     uint4 raw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = load_raw(body + (i + u * kThreads) * W);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float x[W];
-      Vec<T>::unpack(raw[u], x);
-      r.add<W>(x, scale);
-    }
+    for (int u = 0; u < U; ++u) raw[u] = load_raw(body + (int64_t)(i + u * kThreads) * W);
+    r.vectors<T, U>(raw, scale);
   }
   for (; i < vecs; i += kThreads) {
-    float x[W];
-    Vec<T>::unpack(load_raw(body + i * W), x);
-    r.add<W>(x, scale);
+    const uint4 raw[1] = {load_raw(body + (int64_t)i * W)};
+    r.vectors<T, 1>(raw, scale);
   }
-  if (head + vecs * W + threadIdx.x < last) {
-    const float x = load1(z + head + vecs * W + threadIdx.x);
-    r.add<1>(&x, scale);
-  }
-  r = block_join(r, scale, share);
+  if (first + threadIdx.x < head) r.one<T>(load1(z + first + threadIdx.x), scale);
+  const int64_t rest = head + (int64_t)vecs * W + threadIdx.x;
+  if (rest < last) r.one<T>(load1(z + rest), scale);
+  // the entries' maximum and sum go along with the row's
+  const float student = place >= 0 && place < v ? load1(z + place) : 0.f;
+  bool bad = place >= v;
+  Running t;
+  if (place >= 0) t.one<float>(teacher, scale);
+  if (rank == 0)
+    for (int j = threadIdx.x + kThreads; j < e.k; j += kThreads) {
+      const int64_t at = e.index(row, j);
+      bad |= at >= v;
+      if (at >= 0) t.one<float>(e.logit(row, j), scale);
+    }
+  block_join(r, scale, t, scale, share);
   if (parts > 1) {
     if (threadIdx.x == 0) {
       uint32_t at;
@@ -239,27 +270,30 @@ __global__ void __launch_bounds__(kThreads) distill_forward_kernel(const T* logi
     r = Running();
     for (int c = 0; c < parts; ++c) r.join(gathered[c].x, gathered[c].y, scale);
   }
-  const float log_sum = logf(r.sum);
-  // the entries: softmax of the teacher's logits, then the sum of q (ln q - ln p)
-  Running t;
-  for (int j = threadIdx.x; j < e.k; j += kThreads) t.add<1>(&et[j], scale);
-  t = block_join(t, scale, share);
-  const float log_weight = logf(t.sum);
-  float sum = 0.f;
-  for (int j = threadIdx.x; j < e.k; j += kThreads) {
-    if (et[j] == -INFINITY) continue;
-    const float lq = (et[j] - t.top) * inv - log_weight, q = exp2f(lq * kLog2e);
-    // both logs are taken against their maxima, where they are exact to fp32
-    if (!(q <= 0.f)) sum += q * (lq - ((ez[j] - r.top) * inv - log_sum));
+  // the sum of q (ln q - ln p); both logs are taken against their maxima, where they are exact to fp32
+  const float log_sum = logf(r.sum), log_weight = logf(t.sum);
+  auto term = [&](float x, float y) {
+    if (x == -INFINITY) return 0.f;
+    const float lq = (x - t.top) * inv - log_weight, q = exp2f(lq * kLog2e);
+    return q <= 0.f ? 0.f : q * (lq - ((y - r.top) * inv - log_sum));  // (NaN goes through)
+  };
+  float sum = place >= 0 ? term(teacher, student) : 0.f;
+  for (int j = threadIdx.x + kThreads; j < e.k; j += kThreads) {
+    const int64_t at = e.index(row, j);
+    if (at >= 0 && at < v) sum += term(e.logit(row, j), load1(z + at));
   }
-  sum = block_sum(sum, share);
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum;
+  const bool any_bad = __syncthreads_or(bad);
   if (threadIdx.x == 0) {
+    sum = 0.f;
+    for (int w = 0; w < kThreads / 32; ++w) sum += sums[w];
     const float nan = __int_as_float(0x7fffffff);
-    const bool none = t.top == -INFINITY && !(t.sum != t.sum);
-    loss[row] = bad ? nan : none ? 0.f : temperature * temperature * sum;
+    const bool none = t.top == -INFINITY && t.sum == 0.f;
+    loss[row] = any_bad ? nan : none ? 0.f : temperature * temperature * sum;
     stats[3 * row] = r.top;
     stats[3 * row + 1] = r.sum;
-    stats[3 * row + 2] = bad ? nan : none ? -INFINITY : t.top * inv + log_weight;
+    stats[3 * row + 2] = any_bad ? nan : none ? -INFINITY : t.top * inv + log_weight;
   }
 }
 
@@ -288,38 +322,38 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const T* log
     eq[j] = mine ? exp2f((e.logit(row, j) * inv - log_weight) * kLog2e) : 0.f;
   }
   constexpr int W = Vec<T>::n;
-  // x - top is taken first: it is exact where p is not small, and a product rounded before it would not be
   const float weight = up / sum;
-  auto grad = [&](float x) { return none ? 0.f : weight * exp2f((x - top) * scale); };
+  const float neg = -top * scale;
+  auto grad = [&](float x) { return none ? 0.f : weight * exp_from<T>(x, top, neg, scale); };
   const bool same = (((uintptr_t)(z + first) ^ (uintptr_t)(out + first)) & 15) == 0;
   // where the two rows sit differently on their 16-byte lines, every element goes by itself
   const int64_t head = same ? min(last, first + (int64_t)((16 - ((uintptr_t)(z + first) & 15)) & 15) / (int64_t)sizeof(T)) : last;
-  const int64_t vecs = (last - head) / W;
+  const int vecs = (int)((last - head) / W);
   for (int64_t i = first + threadIdx.x; i < head; i += kThreads) out[i] = make1<T>(grad(load1(z + i)));
-  int64_t i = threadIdx.x;
+  int i = threadIdx.x;
   constexpr int U = 4;
   for (; i + (U - 1) * kThreads < vecs; i += U * kThreads) {
     uint4 raw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = load_raw(z + head + (i + u * kThreads) * W);
+    for (int u = 0; u < U; ++u) raw[u] = load_raw(z + head + (int64_t)(i + u * kThreads) * W);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float x[W];
       Vec<T>::unpack(raw[u], x);
 #pragma unroll
       for (int j = 0; j < W; ++j) x[j] = grad(x[j]);
-      store_raw(out + head + (i + u * kThreads) * W, Vec<T>::pack(x));
+      store_raw(out + head + (int64_t)(i + u * kThreads) * W, Vec<T>::pack(x));
     }
   }
   for (; i < vecs; i += kThreads) {
     float x[W];
-    Vec<T>::unpack(load_raw(z + head + i * W), x);
+    Vec<T>::unpack(load_raw(z + head + (int64_t)i * W), x);
 #pragma unroll
     for (int j = 0; j < W; ++j) x[j] = grad(x[j]);
-    store_raw(out + head + i * W, Vec<T>::pack(x));
+    store_raw(out + head + (int64_t)i * W, Vec<T>::pack(x));
   }
-  if (head + vecs * W + threadIdx.x < last) {
-    const int64_t at = head + vecs * W + threadIdx.x;
+  const int64_t at = head + (int64_t)vecs * W + threadIdx.x;
+  if (at < last) {
     out[at] = make1<T>(grad(load1(z + at)));
   }
   __syncthreads();  // the entries' places are written again behind this
@@ -327,7 +361,7 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const T* log
     if (ei[j] < 0) continue;
     float q = 0.f;  // all entries of this place, in order: equal indices write equal values
     for (int m = 0; m < e.k; ++m) q += ei[m] == ei[j] ? eq[m] : 0.f;
-    const float p = exp2f((load1(z + first + ei[j]) - top) * scale) / sum;
+    const float p = exp_from<T>(load1(z + first + ei[j]), top, neg, scale) / sum;
     out[first + ei[j]] = make1<T>(up * (p - q));
   }
 }
@@ -351,13 +385,12 @@ template <typename T>
 int forward_typed(const tcb200_topk_distill_t& p, const void* logits, const Entries& e, float* loss, float* stats,
                   cudaStream_t s) {
   const int sms = sm_count(-1);
-  // clusters while the rows leave the device (two CTAs an SM) idle and a CTA keeps 2048 elements
+  // clusters while the rows make fewer than eight CTAs an SM and a CTA keeps 2048 elements
   int parts = 1;
-  while (parts < kMaxCluster && p.N * parts * 2 <= 2 * sms && p.V / (parts * 2) >= 2048) parts *= 2;
+  while (parts < kMaxCluster && p.N * parts < 8ll * sms && p.V / (parts * 2) >= 2048) parts *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.N * parts));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)p.K * 8;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -376,8 +409,9 @@ template <typename T>
 int backward_typed(const tcb200_topk_distill_t& p, const void* logits, const Entries& e, const float* stats, const float* g,
                    int64_t g_stride, void* dlogits, cudaStream_t s) {
   const int sms = sm_count(-1);
-  // stretches of 2048 elements and more while the rows leave the device (four CTAs an SM) idle
-  const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(4ll * sms / p.N, p.V / 2048));
+  // stretches of at most 32768 elements, and of 2048 and more while the rows make fewer than eight CTAs an SM
+  const int64_t fill = std::min<int64_t>(8ll * sms / p.N, p.V / 2048);
+  const int parts = (int)std::max<int64_t>({1, fill, ceil_div(p.V, 32768)});
   TCB200_CUDA_TRY(launch_pdl(distill_backward_kernel<T>, dim3((unsigned)(p.N * parts)), dim3(kThreads), (size_t)p.K * 8, s,
                              static_cast<const T*>(logits), p.ld_logits, p.V, e, p.temperature, stats, g, g_stride,
                              static_cast<T*>(dlogits), parts));
