@@ -43,14 +43,14 @@ static EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// k-major: box of 64 columns (k) x 128 rows.  mn-major: box of 64 columns (m or n) x 64 rows (k).  Zeros out of bounds.
-int make_map(CUtensorMap* tm, const Operand& o, bool bf16, bool mn_major) {
+// k-major: box of 64 columns (k) x `rows`.  mn-major: box of 64 columns (m or n) x 64 rows (k).  Zeros out of bounds.
+int make_map(CUtensorMap* tm, const Operand& o, bool bf16, bool mn_major, int rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return TCB200_ERR_CUDA;
   cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.planes};
   const int64_t plane = o.planes > 1 ? o.plane_stride : o.rows * o.ld;
   cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)plane * 2};
-  cuuint32_t box[3] = {kBK, (cuuint32_t)(mn_major ? kBK : kHalf), 1};
+  cuuint32_t box[3] = {kBK, (cuuint32_t)(mn_major ? kBK : rows), 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
                   const_cast<void*>(o.base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -265,14 +265,15 @@ struct ForwardEpi {
   float2* part;      // [parts][n_pad]
   float* hit;        // [n_pad] the target's logit
   int64_t n_pad, v0, v, part0;  // first vocabulary entry of this launch, entries of it; number of its first part
-  __device__ void operator()(float (&acc)[128], int row, int col0, int, const CUtensorMap*, const pg::Out&) const {
+  template <int C>
+  __device__ void operator()(float (&acc)[C], int row, int col0, int, const CUtensorMap*, const pg::Out&) const {
     if (row >= head->live || col0 >= v) return;
-    const int have = (int)min(v - col0, (int64_t)128);
+    const int have = (int)min(v - col0, (int64_t)C);
     const int64_t at = (int64_t)target[row] - v0 - col0;
     const int t = at >= 0 && at < have ? (int)at : -1;
     float top = -INFINITY, z = 0.f;
 #pragma unroll
-    for (int j = 0; j < 128; ++j) {
+    for (int j = 0; j < C; ++j) {
       if (j >= have) acc[j] = -INFINITY;
       top = fmaxf(top, acc[j]);
       if (j == t) z = acc[j];
@@ -281,8 +282,8 @@ struct ForwardEpi {
     const float shift = top == -INFINITY ? 0.f : top;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < 128; ++j) sum[j & 3] += exp_neg(acc[j] - shift);
-    part[(part0 + col0 / 128) * n_pad + row] = make_float2(top, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+    for (int j = 0; j < C; ++j) sum[j & 3] += exp_neg(acc[j] - shift);
+    part[(part0 + col0 / C) * n_pad + row] = make_float2(top, (sum[0] + sum[1]) + (sum[2] + sum[3]));
     if (t >= 0) hit[row] = z;
   }
 };
@@ -350,15 +351,16 @@ struct GradEpi {
   const float* share;
   const float* lse;
   int64_t ld, v0, v;
-  __device__ void operator()(float (&acc)[128], int row, int col0, int, const CUtensorMap* tm, const pg::Out& out) const {
+  template <int C>
+  __device__ void operator()(float (&acc)[C], int row, int col0, int, const CUtensorMap* tm, const pg::Out& out) const {
     if (col0 >= ld) return;
     const bool live = row < head->live;
     const float g = live ? share[row] : 0.f, l = live ? lse[row] : 0.f;
     const int64_t at = live ? (int64_t)target[row] - v0 - col0 : -1;
-    const int t = at >= 0 && at < 128 ? (int)at : -1;
-    const int have = live ? (int)min(v - col0, (int64_t)128) : 0;
+    const int t = at >= 0 && at < C ? (int)at : -1;
+    const int have = live ? (int)min(v - col0, (int64_t)C) : 0;
 #pragma unroll
-    for (int c = 0; c < 128; ++c) {
+    for (int c = 0; c < C; ++c) {
       const float d = acc[c] - l;
       const float p = TYPE == kF32 ? expf(d) : exp_neg(d);
       acc[c] = c < have ? g * (c == t ? p - 1.f : p) : 0.f;
@@ -366,7 +368,7 @@ struct GradEpi {
 #pragma unroll
     for (int p = 0; p < (TYPE == kF32 ? 3 : 1); ++p) {
 #pragma unroll
-      for (int h = 0; h < 128; h += 64) {  // a box: 64 columns
+      for (int h = 0; h < C; h += 64) {  // a box: 64 columns
         out.begin();
 #pragma unroll
         for (int c = 0; c < 64; c += 8) {
@@ -395,9 +397,10 @@ struct GradEpi {
 struct SumEpi {
   int64_t ld;  // columns of the sums
   int add;
-  __device__ void operator()(float (&acc)[128], int row, int col0, int split, const CUtensorMap* tm, const pg::Out& out) const {
+  template <int C>
+  __device__ void operator()(float (&acc)[C], int row, int col0, int split, const CUtensorMap* tm, const pg::Out& out) const {
 #pragma unroll
-    for (int h = 0; h < 128; h += 32) {
+    for (int h = 0; h < C; h += 32) {
       if (col0 + h >= ld) return;
       out.begin();
 #pragma unroll
@@ -424,13 +427,14 @@ struct WeightEpi {
   int64_t rows, d;
   float scale;
   int tma;  // rows start on 16-byte boundaries
-  __device__ void operator()(float (&acc)[128], int row, int col0, int, const CUtensorMap* tm, const pg::Out& out) const {
+  template <int C>
+  __device__ void operator()(float (&acc)[C], int row, int col0, int, const CUtensorMap* tm, const pg::Out& out) const {
     const int row0 = row - out.lane;
     if (row0 >= rows) return;
     const float k = head->gscale * scale;
     constexpr int W = 16 / sizeof(T), COLS = 128 / sizeof(T);
 #pragma unroll
-    for (int h = 0; h < 128; h += COLS) {
+    for (int h = 0; h < C; h += COLS) {
       if (col0 + h >= d) return;
       out.begin();
 #pragma unroll
@@ -502,7 +506,8 @@ constexpr int64_t kPieceBytes = 256ll << 20;  // dZ of a piece, and a packed pie
 struct Layout {
   int64_t n_pad, dp, planes;
   int64_t fwd_piece, bwd_piece;  // vocabulary entries per piece
-  int64_t parts;
+  int64_t parts;                 // of a row's logits, one per drain warp's columns
+  int fwd_bn, bwd_bn, dw_bn;     // columns of a tile: logits forward, logits backward, dW
   int splits;
   int64_t fwd_bytes, bwd_bytes;
   // byte offsets
@@ -532,12 +537,16 @@ int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
   };
   l->fwd_piece = pack_w(p) ? piece(l->dp * 2 * l->planes) : v_pad;
   l->bwd_piece = piece(2 * l->planes * (pack_w(p) ? std::max(l->dp, l->n_pad) : l->n_pad));
-  l->parts = ceil_div(p.V, 128);
+  const int products = l->planes == 3 ? 6 : 1;
+  l->fwd_bn = pg::tile_columns(l->n_pad, l->fwd_piece, p.D, products, sms);
+  l->bwd_bn = pg::tile_columns(l->n_pad, l->bwd_piece, p.D, products, sms);
+  l->dw_bn = pg::tile_columns(l->bwd_piece, p.D, p.N, products, sms);
+  l->parts = ceil_div(p.V, l->fwd_bn / 2);
   // dX has few tiles and a long sum: the vocabulary of a piece is split where that fills the last round of the pairs.
   // Cost of S splits in k-blocks of a pair: rounds x (a unit's k-blocks + 8 for its start and epilogue) + what adding S
   // planes costs (a plane of a tile is about 4 k-blocks of memory traffic).
   const int64_t tiles = (l->n_pad / kTile) * ceil_div(p.D, kTile), pairs = std::max(1, sms / 2);
-  const int64_t kb = ceil_div(l->bwd_piece, pg::kBK) * (l->planes == 3 ? 6 : 1);
+  const int64_t kb = ceil_div(l->bwd_piece, pg::kBK) * products;
   int64_t best = INT64_MAX;
   l->splits = 1;
   for (int64_t s = 1; s <= 64 && s * 8 <= kb; ++s) {
@@ -666,7 +675,7 @@ int backward_typed(const tcb200_linear_ce_t& p, const Layout& l, const void* W, 
     const GradEpi<TYPE> ge{r.head, r.target, r.share, r.lse, ld, v0, v};
     CUtensorMap tc;
     if ((st = pg::make_out_map(&tc, {dz, ld, l.n_pad, ld, l.planes, l.n_pad * ld}, 2)) != TCB200_OK) return st;
-    st = pg::launch<false, false>(x, w, bf16, gemm_args(l, p.N, v, p.D, &r.head->live, 0, status, false), tc, ge, device, sms, s);
+    st = pg::launch_columns<false, false>(l.bwd_bn, x, w, bf16, gemm_args(l, p.N, v, p.D, &r.head->live, 0, status, false), tc, ge, device, sms, s);
     if (st != TCB200_OK) return st;
     const pg::Operand z{dz, v, l.n_pad, ld, l.planes, l.n_pad * ld};
     if (dX) {
@@ -676,14 +685,14 @@ int backward_typed(const tcb200_linear_ce_t& p, const Layout& l, const void* W, 
       pg::Args a = gemm_args(l, p.N, p.D, v, &r.head->live, 0, status, false);
       a.splits = l.splits;
       a.split_kb = (int)ceil_div(ceil_div(v, pg::kBK), l.splits);
-      if ((st = pg::launch<false, true>(z, w, bf16, a, tc, se, device, sms, s)) != TCB200_OK) return st;
+      if ((st = pg::launch<256, false, true>(z, w, bf16, a, tc, se, device, sms, s)) != TCB200_OK) return st;
     }
     if (dW) {
       T* out = dW + v0 * p.D;
       const int tma = (p.D * sizeof(T)) % 16 == 0 && ((uintptr_t)out & 15) == 0;
       if (tma && (st = pg::make_out_map(&tc, {out, p.D, v, p.D, 1, 0}, sizeof(T))) != TCB200_OK) return st;
       const WeightEpi<T> we{r.head, out, v, p.D, scale, tma};
-      st = pg::launch<true, true>(z, x, bf16, gemm_args(l, v, p.D, p.N, &r.head->live, 1, status, false), tc, we, device, sms, s);
+      st = pg::launch_columns<true, true>(l.dw_bn, z, x, bf16, gemm_args(l, v, p.D, p.N, &r.head->live, 1, status, false), tc, we, device, sms, s);
       if (st != TCB200_OK) return st;
     }
   }
@@ -735,8 +744,8 @@ int tcb200_linear_ce_forward(const tcb200_linear_ce_t* problem, const void* X, c
     const int64_t v = std::min(l.fwd_piece, p.V - v0);
     pg::Operand w;
     if ((st = w_operand(p, l, W, v0, v, l.fwd_piece, ws + l.w_fwd, sms, s, &w)) != TCB200_OK) return st;
-    const ForwardEpi e{r.head, r.target, part, hit, l.n_pad, v0, v, v0 / 128};
-    st = pg::launch<false, false>(x, w, p.dtype != TCB200_F16, gemm_args(l, p.N, v, p.D, &r.head->live, 0, status, true),
+    const ForwardEpi e{r.head, r.target, part, hit, l.n_pad, v0, v, v0 / (l.fwd_bn / 2)};
+    st = pg::launch_columns<false, false>(l.fwd_bn, x, w, p.dtype != TCB200_F16, gemm_args(l, p.N, v, p.D, &r.head->live, 0, status, true),
                                   CUtensorMap{}, e, device, sms, s);
     if (st != TCB200_OK) return st;
   }

@@ -1,6 +1,6 @@
 // 16-bit matrix products on CTA pairs with fp32 accuracy of the sum, shared by the kernels of the large-vocabulary
-// losses (sm_100a).  One pair computes a 256 x 256 tile C(m, n) = sum_k A(m, k) B(n, k); the epilogue is a functor that
-// gets a row and 128 consecutive columns of it in registers.
+// losses (sm_100a).  One pair computes a tile C(m, n) = sum_k A(m, k) B(n, k) of 256 rows and BN = 256 or 128 columns; the
+// epilogue is a functor that gets a row and BN / 2 consecutive columns of it in registers.
 //
 // Operands are f16 or bf16 (both the same), each either k-major (rows of k) or mn-major (rows of m or n): the three
 // products of a linear layer's training step (X W^T, dZ W, dZ^T X) then read the same arrays without a transposed copy.
@@ -8,7 +8,7 @@
 // the six with i + j <= 2 are summed, smallest first, and the largest dropped one is 2^-24 of the product.
 //
 // Roles of a CTA: warps 0-7 drain the accumulator and run the epilogue, warp 8 issues the TMA loads of this CTA's
-// 128 rows of A and 128 of the tile's 256 rows of B, the leader's warp 9 issues the MMAs (M = 256, N = 256, K = 16) of both
+// 128 rows of A and BN / 2 of the tile's BN rows of B, the leader's warp 9 issues the MMAs (M = 256, N = BN, K = 16) of both
 // CTAs.  In both issuing warps all lanes run the loop and one elected lane issues, so that descriptors and addresses stay in
 // uniform registers.  With loops that only lane 0 ran, a k-block's loads took 400 cycles to issue and its four MMAs 300, and a
 // k-block 740 cycles where its MMAs take 512 (4096 x 2048 x 32000, forward: 393 us; now 332 us, 1.62 PFLOP/s).  Of the rest
@@ -25,8 +25,8 @@
 namespace tcb200 {
 namespace pg {
 
-constexpr int kTile = 256;      // tile rows and columns of a pair
-constexpr int kHalf = 128;      // rows of A, and of B, that one CTA loads
+constexpr int kTile = 256;      // tile rows of a pair, and its columns at most
+constexpr int kHalf = 128;      // rows of A, and of B at most, that one CTA loads
 constexpr int kBK = 64;         // k of a stage: one 128-byte swizzle row of 16-bit values
 constexpr int kOperandBytes = kHalf * kBK * 2;
 constexpr int kStageBytes = 2 * kOperandBytes;
@@ -97,18 +97,18 @@ template <bool MN>
 __host__ __device__ constexpr uint32_t k_step_bytes() { return MN ? 16 * 128 : 32; }
 
 // kind::f16: D = f32, A = B = f16 (bf16 = 0) or bf16, each k-major or mn-major.
-__host__ inline uint32_t make_idesc(bool bf16, bool a_mn, bool b_mn) {
+__host__ inline uint32_t make_idesc(bool bf16, bool a_mn, bool b_mn, int bn) {
   const uint32_t t = bf16 ? 1 : 0;
   return (1u << 4) | (t << 7) | (t << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
-         ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+         ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
 }
 
-// One operand stage of this CTA: 128 rows of m (or n) from mn0, 64 k from k0.
-template <bool MN>
+// One operand stage of this CTA: ROWS (128 or 64) rows of m (or n) from mn0, 64 k from k0.
+template <bool MN, int ROWS>
 __device__ __forceinline__ void load_operand(uint8_t* dst, const CUtensorMap* tm, int mn0, int k0, int plane, uint32_t bar) {
   if (MN) {
     tma_load_3d_pair(dst, tm, mn0, k0, plane, bar);
-    tma_load_3d_pair(dst + kBK * 128, tm, mn0 + 64, k0, plane, bar);
+    if (ROWS > 64) tma_load_3d_pair(dst + kBK * 128, tm, mn0 + 64, k0, plane, bar);
   } else {
     tma_load_3d_pair(dst, tm, k0, mn0, plane, bar);
   }
@@ -119,11 +119,11 @@ __device__ __forceinline__ void load_operand(uint8_t* dst, const CUtensorMap* tm
 struct Units {
   int64_t tiles_m, tiles_n, units;
   int kb, splits, split_kb;
-  __device__ Units(const Args& a) {
+  __device__ Units(const Args& a, int bn) {
     int64_t M = a.M, K = a.K;
     if (a.live) (a.live_is_k ? K : M) = *a.live;
     tiles_m = (M + kTile - 1) / kTile;
-    tiles_n = (a.N + kTile - 1) / kTile;
+    tiles_n = (a.N + bn - 1) / bn;
     kb = (int)((K + kBK - 1) / kBK);
     splits = a.splits;
     split_kb = a.split_kb > 0 ? a.split_kb : kb;
@@ -184,12 +184,15 @@ struct Out {
   }
 };
 
-// Epi: struct with  __device__ void operator()(float (&acc)[128], int row, int col0, int split, const CUtensorMap* tm,
-// const Out& out)  where row and col0 are the thread's row and first column of C (both may lie outside it).
-template <bool A_MN, bool B_MN, class Epi>
+// Epi: struct with  template <int C> __device__ void operator()(float (&acc)[C], int row, int col0, int split,
+// const CUtensorMap* tm, const Out& out)  where row and col0 are the thread's row and first of its C = BN / 2 columns (both
+// may lie outside the result).
+template <int BN, bool A_MN, bool B_MN, class Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                  const __grid_constant__ CUtensorMap tmC, const __grid_constant__ Args a, const __grid_constant__ Epi epi) {
+  static_assert(BN == 256 || BN == 128, "an operand's mn-major rows are whole 64-element groups in each CTA");
+  constexpr int C = BN / 2;  // columns of a drain warp; rows of B that this CTA loads
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kBarrierOffset);  // used in the leader: both CTAs' loads
@@ -223,7 +226,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   pdl_sync();
   const uint32_t tmem_base = *tmem_slot;
 
-  const Units units(a);
+  const Units units(a, BN);
 
   if (warp == kDrainWarps) {
     // ------------------------------------------------ TMA producer
@@ -236,7 +239,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       int64_t tm, tn;
       int split, kb0, nkb;
       units.locate(u, &tm, &tn, &split, &kb0, &nkb);
-      const int m0 = (int)(tm * kTile) + (int)rank * kHalf, n0 = (int)(tn * kTile) + (int)rank * kHalf;
+      const int m0 = (int)(tm * kTile) + (int)rank * kHalf, n0 = (int)(tn * BN) + (int)rank * C;
       for (int c0 = 0; c0 < nkb && ok; c0 += a.chunk_kb) {
         const int c1 = c0 + a.chunk_kb < nkb ? c0 + a.chunk_kb : nkb;
         for (int p = 0; p < a.products && ok; ++p)
@@ -244,10 +247,10 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             ok = mbar_wait(&empty[s], phase, 21, a.dev_status, abort_flag);
             if (!ok) break;
             if (issuer) {
-              if (rank == 0) mbar_expect_tx(&full[s], 2 * kStageBytes);
+              if (rank == 0) mbar_expect_tx(&full[s], 2 * (kOperandBytes + C * kBK * 2));
               uint8_t* dst = smem + s * kStageBytes;
-              load_operand<A_MN>(dst, &tmA, m0, (kb0 + kb) * kBK, a.pa[p], full0 + s * 8);
-              load_operand<B_MN>(dst + kOperandBytes, &tmB, n0, (kb0 + kb) * kBK, a.pb[p], full0 + s * 8);
+              load_operand<A_MN, kHalf>(dst, &tmA, m0, (kb0 + kb) * kBK, a.pa[p], full0 + s * 8);
+              load_operand<B_MN, C>(dst + kOperandBytes, &tmB, n0, (kb0 + kb) * kBK, a.pb[p], full0 + s * 8);
             }
             __syncwarp();
             if (++s == kStages) {
@@ -302,7 +305,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     }
   } else {
     // ------------------------------------------------ drain + epilogue
-    const int q = warp & 3, half = warp >> 2;  // tensor-memory lane quarter; which 128 of the 256 columns
+    const int q = warp & 3, half = warp >> 2;  // tensor-memory lane quarter; which half of the columns
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
     const Out out{smem + kOutOffset + warp * kOutBytes, lane};
     uint32_t chunk = 0;
@@ -311,20 +314,20 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       int64_t tm, tn;
       int split, kb0, nkb;
       units.locate(u, &tm, &tn, &split, &kb0, &nkb);
-      float acc[128];
+      float acc[C];
 #pragma unroll
-      for (int j = 0; j < 128; ++j) acc[j] = 0.f;
+      for (int j = 0; j < C; ++j) acc[j] = 0.f;
       for (int c0 = 0; c0 < nkb; c0 += a.chunk_kb, ++chunk) {
         const int b = chunk & 1;
         ok = mbar_wait(&acc_full[b], (chunk >> 1) & 1, 24, a.dev_status, abort_flag);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
-        for (int g = 0; g < 8; ++g) {
+        for (int g = 0; g < C / 16; ++g) {
           float v[16];
-          tmem_ld16_nowait(tmem_base + b * kTile + lane_base + half * 128 + g * 16, v);
+          tmem_ld16_nowait(tmem_base + b * kTile + lane_base + half * C + g * 16, v);
           tmem_wait_ld();
-          if (g == 7) {
+          if (g == C / 16 - 1) {
             tc_fence_before();
             mbar_arrive_warp_remote(&acc_empty[b], 0);
           }
@@ -333,7 +336,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         }
       }
       if (!ok) break;
-      epi(acc, (int)(tm * kTile) + (int)rank * kHalf + q * 32 + lane, (int)(tn * kTile) + half * 128, split, &tmC, out);
+      epi(acc, (int)(tm * kTile) + (int)rank * kHalf + q * 32 + lane, (int)(tn * BN) + half * C, split, &tmC, out);
     }
     if (lane == 0) tma_store_wait_all();
   }
@@ -353,30 +356,46 @@ struct Operand {
   const void* base;
   int64_t cols, rows, ld, planes, plane_stride;
 };
-int make_map(CUtensorMap* tm, const Operand& o, bool bf16, bool mn_major);
+int make_map(CUtensorMap* tm, const Operand& o, bool bf16, bool mn_major, int rows);
 // An output [planes][rows][cols] of 2- or 4-byte elements, written in boxes of 32 rows x 128 bytes.
 int make_out_map(CUtensorMap* tm, const Operand& o, int bytes);
 
-template <bool A_MN, bool B_MN, class Epi>
+// Columns of a tile: 128 where that finishes earlier, which is where tiles of 256 leave pairs without work.  A k-block takes a
+// pair about 530 cycles with 256 columns and 400 with 128 (the loads, not the MMAs, bound it then); a unit's start, drain
+// and epilogue about 6000 and 4000.
+inline int tile_columns(int64_t M, int64_t N, int64_t K, int products, int sms) {
+  const int64_t pairs = std::max(1, sms / 2), tiles_m = ceil_div(M, kTile), steps = ceil_div(K, kBK) * products;
+  const int64_t wide = ceil_div(tiles_m * ceil_div(N, 256), pairs) * (530 * steps + 6000);
+  const int64_t narrow = ceil_div(tiles_m * ceil_div(N, 128), pairs) * (400 * steps + 4000);
+  return narrow < wide ? 128 : 256;
+}
+
+template <int BN, bool A_MN, bool B_MN, class Epi>
 int launch(const Operand& A, const Operand& B, bool bf16, Args args, const CUtensorMap& tc, const Epi& epi, int device, int sms,
            cudaStream_t s) {
   CUtensorMap ta, tb;
-  int st = make_map(&ta, A, bf16, A_MN);
-  if (st == TCB200_OK) st = make_map(&tb, B, bf16, B_MN);
+  int st = make_map(&ta, A, bf16, A_MN, kHalf);
+  if (st == TCB200_OK) st = make_map(&tb, B, bf16, B_MN, BN / 2);
   if (st != TCB200_OK) return st;
-  args.idesc = make_idesc(bf16, A_MN, B_MN);
+  args.idesc = make_idesc(bf16, A_MN, B_MN, BN);
   if (args.products == 1) args.pa[0] = args.pb[0] = 0;
   else {
     const int pa[6] = {2, 1, 0, 1, 0, 0}, pb[6] = {0, 1, 2, 0, 1, 0};
     for (int i = 0; i < 6; ++i) args.pa[i] = pa[i], args.pb[i] = pb[i];
   }
-  const int64_t units = ceil_div(args.M, kTile) * ceil_div(args.N, kTile) * args.splits;
+  const int64_t units = ceil_div(args.M, kTile) * ceil_div(args.N, BN) * args.splits;
   if (units == 0) return TCB200_OK;
   const unsigned pairs = (unsigned)std::min<int64_t>(units, std::max(1, sms / 2));
   static std::atomic<uint64_t> configured{0};
-  TCB200_CUDA_TRY(ensure_dynamic_smem(pair_gemm_kernel<A_MN, B_MN, Epi>, kSmemBytes, device, configured));
-  TCB200_CUDA_TRY(launch_pdl(pair_gemm_kernel<A_MN, B_MN, Epi>, dim3(2 * pairs), dim3(kThreads), kSmemBytes, s, ta, tb, tc, args, epi));
+  TCB200_CUDA_TRY(ensure_dynamic_smem(pair_gemm_kernel<BN, A_MN, B_MN, Epi>, kSmemBytes, device, configured));
+  TCB200_CUDA_TRY(launch_pdl(pair_gemm_kernel<BN, A_MN, B_MN, Epi>, dim3(2 * pairs), dim3(kThreads), kSmemBytes, s, ta, tb, tc, args, epi));
   return TCB200_OK;
+}
+template <bool A_MN, bool B_MN, class Epi>
+int launch_columns(int bn, const Operand& A, const Operand& B, bool bf16, const Args& args, const CUtensorMap& tc, const Epi& epi,
+                   int device, int sms, cudaStream_t s) {
+  return bn == 128 ? launch<128, A_MN, B_MN, Epi>(A, B, bf16, args, tc, epi, device, sms, s)
+                   : launch<256, A_MN, B_MN, Epi>(A, B, bf16, args, tc, epi, device, sms, s);
 }
 
 }  // namespace pg
