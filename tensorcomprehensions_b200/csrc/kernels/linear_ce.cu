@@ -11,13 +11,11 @@
 //
 // Rows are compacted first: rows without a target (target == ignore_index) cost nothing, and what their X holds, infinities
 // and NaN included, is never read.  The number of rows that remain stays on the device (pg::Args::live).
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <math.h>
 #include <string.h>
 
 #include <mutex>
 
+#include "linear_ce.cuh"
 #include "pair_gemm.cuh"
 
 namespace tcb200 {
@@ -75,32 +73,13 @@ int make_out_map(CUtensorMap* tm, const Operand& o, int bytes) {
 
 }  // namespace pg
 
+using namespace lce;
+
 namespace {
 
 using pg::kTile;
 
-// What the kernels share besides the operands, at the head of the workspace.
-struct Head {
-  int live;      // rows with a target
-  int status;    // a bounded wait that gave up
-  float gscale;  // largest |g| of the live rows
-};
-
-// ---- rows -----------------------------------------------------------------------------------------------------------
-struct Rows {
-  Head* head;
-  int* place;     // [n] row -> live row, -1 without a target
-  int* target;    // [n_pad] of a live row; -1: outside [0, V)
-  float* share;   // [n_pad] g of a live row / gscale (backward)
-  float* lse;     // [n_pad] of a live row (backward)
-};
-
 // ---- operands -------------------------------------------------------------------------------------------------------
-template <typename T>
-__device__ __forceinline__ float to_float(T v);
-template <> __device__ __forceinline__ float to_float(float v) { return v; }
-template <> __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-
 __device__ __forceinline__ uint16_t bits(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
 __device__ __forceinline__ uint16_t bits(__half v) { return __half_as_ushort(v); }
 
@@ -253,11 +232,6 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const Index* target, 
 }
 
 // ---- epilogues ------------------------------------------------------------------------------------------------------
-constexpr float kLog2e = 1.4426950408889634f;
-
-// exp(x), x <= 0: the base-2 exponential of the hardware; the product rounds x log2(e) to 2^-24 of itself
-__device__ __forceinline__ float exp_neg(float x) { return exp2f(x * kLog2e); }
-
 // Forward: maximum and sum of exp(z - maximum) over this thread's columns, and the target's logit.
 struct ForwardEpi {
   const Head* head;
@@ -290,15 +264,6 @@ struct ForwardEpi {
 
 // Joins the parts of a row: lse, and the loss lse - z_target.  32 rows x 32 lanes of parts a block, four loads in flight a
 // thread; a row's parts are joined in a fixed order.
-struct Running {
-  float top = -INFINITY, sum = 0.f;
-  __device__ __forceinline__ void join(float2 x) {
-    // fmaxf drops a NaN maximum; its sum is NaN then too and survives
-    const float m = fmaxf(top, x.x), shift = m == -INFINITY ? 0.f : m;
-    sum = sum * exp_neg(top - shift) + x.y * exp_neg(x.x - shift);
-    top = m;
-  }
-};
 __global__ void __launch_bounds__(1024) join_kernel(Rows r, const float2* part, const float* hit, int64_t parts,
                                                     int64_t n_pad, int64_t n, float* loss, float* lse, int* dev_status) {
   __shared__ float2 share[32][33];
@@ -413,12 +378,6 @@ struct SumEpi {
   }
 };
 
-template <typename T>
-__device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ float from_float(float v) { return v; }
-template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
-
 // dW of a piece: whole sums, scaled and rounded once.
 template <typename T>
 struct WeightEpi {
@@ -478,6 +437,7 @@ __global__ void __launch_bounds__(256) finish_kernel(Rows r, const float* sums, 
     const int at = r.place[row];
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (at >= 0) {
+#pragma unroll 4
       for (int s = 0; s < splits; ++s) {
         const float4* p = reinterpret_cast<const float4*>(sums + s * plane + at * ld + c);
         const float4 a = p[0], b = p[1];
@@ -504,11 +464,12 @@ __global__ void __launch_bounds__(256) finish_kernel(Rows r, const float* sums, 
 constexpr int64_t kPieceBytes = 256ll << 20;  // dZ of a piece, and a packed piece of W
 
 struct Layout {
-  int64_t n_pad, dp, planes;
+  int64_t n_pad, dp, planes, sum_rows;
   int64_t fwd_piece, bwd_piece;  // vocabulary entries per piece
   int64_t parts;                 // of a row's logits, one per drain warp's columns
   int fwd_bn, bwd_bn, dw_bn;     // columns of a tile: logits forward, logits backward, dW
-  int splits;
+  int splits;                    // planes of partial sums of dX
+  bool few_fwd, few_bwd;         // the kernels for few rows: nothing is packed, no dZ is kept
   int64_t fwd_bytes, bwd_bytes;
   // byte offsets
   int64_t place, target, share, lse, hit, part, x, w_fwd, w_bwd, dz, sums;
@@ -541,7 +502,9 @@ int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
   l->fwd_bn = pg::tile_columns(l->n_pad, l->fwd_piece, p.D, products, sms);
   l->bwd_bn = pg::tile_columns(l->n_pad, l->bwd_piece, p.D, products, sms);
   l->dw_bn = pg::tile_columns(l->bwd_piece, p.D, p.N, products, sms);
-  l->parts = ceil_div(p.V, l->fwd_bn / 2);
+  l->few_fwd = few_forward_ok(p);
+  l->few_bwd = few_backward_ok(p);
+  l->parts = l->few_fwd ? few_blocks(p, sms) : ceil_div(p.V, l->fwd_bn / 2);
   // dX has few tiles and a long sum: the vocabulary of a piece is split where that fills the last round of the pairs.
   // Cost of S splits in k-blocks of a pair: rounds x (a unit's k-blocks + 8 for its start and epilogue) + what adding S
   // planes costs (a plane of a tile is about 4 k-blocks of memory traffic).
@@ -556,6 +519,7 @@ int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
       l->splits = (int)s;
     }
   }
+  if (l->few_bwd) l->splits = (int)few_blocks(p, sms);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t here = at;
@@ -567,16 +531,17 @@ int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
   l->target = take(l->n_pad * 4);
   l->share = take(l->n_pad * 4);
   l->lse = take(l->n_pad * 4);
-  l->x = take(l->planes * l->n_pad * l->dp * 2);
+  l->x = take(l->few_fwd && l->few_bwd ? 0 : l->planes * l->n_pad * l->dp * 2);
   const int64_t common = at;
   l->hit = take(l->n_pad * 4);
   l->part = take(l->parts * l->n_pad * 8);
-  l->w_fwd = take(pack_w(p) ? l->planes * l->fwd_piece * l->dp * 2 : 0);
+  l->w_fwd = take(pack_w(p) && !l->few_fwd ? l->planes * l->fwd_piece * l->dp * 2 : 0);
   l->fwd_bytes = at;
   at = common;
-  l->w_bwd = take(pack_w(p) ? l->planes * l->bwd_piece * l->dp * 2 : 0);
-  l->dz = take(l->planes * l->n_pad * l->bwd_piece * 2);
-  l->sums = take((int64_t)l->splits * l->n_pad * l->dp * 4);
+  l->w_bwd = take(pack_w(p) && !l->few_bwd ? l->planes * l->bwd_piece * l->dp * 2 : 0);
+  l->dz = take(l->few_bwd ? 0 : l->planes * l->n_pad * l->bwd_piece * 2);
+  l->sum_rows = l->few_bwd ? kFewRows : l->n_pad;
+  l->sums = take((int64_t)l->splits * l->sum_rows * l->dp * 4);
   l->bwd_bytes = at;
   return TCB200_OK;
 }
@@ -735,12 +700,13 @@ int tcb200_linear_ce_forward(const tcb200_linear_ce_t* problem, const void* X, c
   char* ws = static_cast<char*>(workspace);
   const Rows r = rows_of(ws, l);
   int* status = &r.head->status;
-  st = launch_rows(p, l, X, target, nullptr, 0, nullptr, r, ws + l.x, sms, s);
-  if (st != TCB200_OK) return st;
-  const pg::Operand x{ws + l.x, l.dp, l.n_pad, l.dp, l.planes, l.n_pad * l.dp};
   float2* part = reinterpret_cast<float2*>(ws + l.part);
   float* hit = reinterpret_cast<float*>(ws + l.hit);
-  for (int64_t v0 = 0; v0 < p.V; v0 += l.fwd_piece) {
+  st = l.few_fwd ? few_forward(p, X, W, target, r, part, hit, l.n_pad, device, sms, s)
+                 : launch_rows(p, l, X, target, nullptr, 0, nullptr, r, ws + l.x, sms, s);
+  if (st != TCB200_OK) return st;
+  const pg::Operand x{ws + l.x, l.dp, l.n_pad, l.dp, l.planes, l.n_pad * l.dp};
+  for (int64_t v0 = l.few_fwd ? p.V : 0; v0 < p.V; v0 += l.fwd_piece) {
     const int64_t v = std::min(l.fwd_piece, p.V - v0);
     pg::Operand w;
     if ((st = w_operand(p, l, W, v0, v, l.fwd_piece, ws + l.w_fwd, sms, s, &w)) != TCB200_OK) return st;
@@ -776,6 +742,9 @@ int tcb200_linear_ce_backward(const tcb200_linear_ce_t* problem, const void* X, 
   char* ws = static_cast<char*>(workspace);
   const Rows r = rows_of(ws, l);
   int* status = &r.head->status;
+  if (l.few_bwd)
+    return few_backward(p, X, W, target, lse, grad_loss, grad_stride, r, reinterpret_cast<float*>(ws + l.sums),
+                        l.sum_rows * l.dp, l.dp, dX, dW, device, sms, s);
   st = launch_rows(p, l, X, target, grad_loss, grad_stride, lse, r, ws + l.x, sms, s);
   if (st != TCB200_OK) return st;
   switch (p.dtype) {

@@ -1,0 +1,69 @@
+// What the kernels of the linear layer's cross entropy share.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math.h>
+
+#include "common.cuh"
+
+namespace tcb200 {
+namespace lce {
+
+// What the kernels share besides the operands, at the head of the workspace.
+struct Head {
+  int live;      // rows with a target
+  int status;    // a bounded wait that gave up
+  float gscale;  // largest |g| of the live rows
+};
+
+struct Rows {
+  Head* head;
+  int* place;     // [n] row -> live row, -1 without a target
+  int* target;    // [n_pad] of a live row; -1: outside [0, V)
+  float* share;   // [n_pad] g of a live row / gscale (backward)
+  float* lse;     // [n_pad] of a live row (backward)
+};
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v);
+template <> __device__ __forceinline__ float to_float(float v) { return v; }
+template <> __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+
+template <> __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// exp(x), x <= 0: the base-2 exponential of the hardware; the product rounds x log2(e) to 2^-24 of itself
+__device__ __forceinline__ float exp_neg(float x) { return exp2f(x * kLog2e); }
+
+// Running maximum and sum of exp(z - maximum).  An empty pair is (-inf, 0).
+struct Running {
+  float top = -INFINITY, sum = 0.f;
+  __device__ __forceinline__ void join(float2 x) {
+    // fmaxf drops a NaN maximum; its sum is NaN then too and survives
+    const float m = fmaxf(top, x.x), shift = m == -INFINITY ? 0.f : m;
+    sum = sum * exp_neg(top - shift) + x.y * exp_neg(x.x - shift);
+    top = m;
+  }
+};
+// Few rows (linear_ce_few.cu): whether they take a problem, the pairs of a row (or the planes of dX) that they leave, and the
+// launches.  `place` and `target` of the rows, the head and the pairs are written as the other path's kernels write them.
+constexpr int kFewRows = 8;
+bool few_forward_ok(const tcb200_linear_ce_t& p);
+bool few_backward_ok(const tcb200_linear_ce_t& p);
+int64_t few_blocks(const tcb200_linear_ce_t& p, int sms);
+int few_forward(const tcb200_linear_ce_t& p, const void* X, const void* W, const void* target, const Rows& r, float2* part,
+                float* hit, int64_t n_pad, int device, int sms, cudaStream_t s);
+int few_backward(const tcb200_linear_ce_t& p, const void* X, const void* W, const void* target, const float* lse,
+                 const float* g, int64_t g_stride, const Rows& r, float* sums, int64_t plane, int64_t ld, void* dX, void* dW,
+                 int device, int sms, cudaStream_t s);
+
+}  // namespace lce
+}  // namespace tcb200

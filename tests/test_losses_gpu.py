@@ -88,6 +88,32 @@ def test_linear_cross_entropy(cuda, dtype, n, d, v, ignored):
     check_ce(x, w, t, up, *step_ce(x, w, t, up))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,d,v,ignored", [
+    (1, 1024, 32000, 0), (1, 20000, 300, 0), (2, 96, 31, 0), (4, 1000, 3001, 0.3), (5, 77, 40000, 0), (8, 512, 9999, 0.3), (8, 2500, 700, 0),
+    (8, 4096, 500, 0), (3, 8200, 257, 0), (7, 333, 33, 0.5), (9, 1000, 3001, 0)])
+def test_few_rows(cuda, dtype, n, d, v, ignored):
+    x, w, t, up = make_ce(cuda, n, d, v, dtype, ignored, seed=n * d + v)
+    t[n // 2] = v - 1
+    got = step_ce(x, w, t, up)
+    check_ce(x, w, t, up, *got)
+    # rows of W off the 16-byte boundaries: the same products in another order
+    ws = torch.full((v, d + 1), float("nan"), device=cuda, dtype=dtype)[:, 1:]
+    ws.copy_(w)
+    check_ce(x, ws, t, up, *step_ce(x, ws, t, up))
+    # masked rows hold anything; a target outside is NaN
+    if (t == -100).any():
+        x2, up2 = x.clone(), up.clone()
+        x2[t == -100] = float("inf")
+        up2[t == -100] = float("nan")
+        for a, b in zip(got, step_ce(x2, w, t, up2)):
+            assert torch.equal(a, b)
+    t2 = t.clone()
+    t2[0] = v
+    loss, dx, dw = step_ce(x, w, t2, up)
+    assert loss[0].isnan() and dx[0].isnan().all() and dw.isnan().all() and dx[1:].isfinite().all()
+
+
 @pytest.mark.parametrize("dtype,n,d,v", [(torch.bfloat16, 4000, 40, 40000), (torch.float32, 1000, 33, 50000), (torch.float16, 2050, 41, 70001)])
 def test_several_pieces_of_the_vocabulary(cuda, dtype, n, d, v):
     x, w, t, up = make_ce(cuda, n, d, v, dtype, 0.1, seed=5)
