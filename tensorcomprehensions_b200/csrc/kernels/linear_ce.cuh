@@ -53,9 +53,9 @@ struct Running {
     top = m;
   }
 };
-// Few rows (linear_ce_few.cu): whether they take a problem, the pairs of a row (or the planes of dX) that they leave, and the
+// Few rows (linear_ce_few.cu): whether its kernels take a problem, the pairs of a row (or the planes of dX) that they leave, and the
 // launches.  `place` and `target` of the rows, the head and the pairs are written as the other path's kernels write them.
-constexpr int kFewRows = 8;
+constexpr int kFewRows = 16;
 bool few_forward_ok(const tcb200_linear_ce_t& p);
 bool few_backward_ok(const tcb200_linear_ce_t& p);
 int64_t few_blocks(const tcb200_linear_ce_t& p, int sms);

@@ -91,7 +91,7 @@ def test_linear_cross_entropy(cuda, dtype, n, d, v, ignored):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,d,v,ignored", [
     (1, 1024, 32000, 0), (1, 20000, 300, 0), (2, 96, 31, 0), (4, 1000, 3001, 0.3), (5, 77, 40000, 0), (8, 512, 9999, 0.3), (8, 2500, 700, 0),
-    (8, 4096, 500, 0), (3, 8200, 257, 0), (7, 333, 33, 0.5), (9, 1000, 3001, 0)])
+    (8, 4096, 500, 0), (3, 8200, 257, 0), (7, 333, 33, 0.5), (9, 1000, 3001, 0), (16, 705, 4000, 0.2), (13, 64, 130, 0), (17, 100, 300, 0)])
 def test_few_rows(cuda, dtype, n, d, v, ignored):
     x, w, t, up = make_ce(cuda, n, d, v, dtype, ignored, seed=n * d + v)
     t[n // 2] = v - 1
