@@ -83,12 +83,24 @@ using pg::kTile;
 __device__ __forceinline__ uint16_t bits(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
 __device__ __forceinline__ uint16_t bits(__half v) { return __half_as_ushort(v); }
 
-// v = p0 + p1 + p2, each the bf16 nearest to what is left: 24 significand bits and more.  A value without a finite
-// remainder (infinite, NaN) is carried by p0 alone.
+// float32 operands.  The logits take two f16 planes of the row scaled by a power of two, v 2^e = h0 + h1: the row's largest
+// value lies in [2^14, 2^15), values down to 2^-17 of it keep 22 significand bits and smaller ones 2^-40 of it.  Three
+// products h1 h0 + h0 h1 + h0 h0 then give z to fp32's accuracy, half of what bf16 planes need, and 2^-e is taken off in the
+// epilogue.  The gradient's products sum over the rows that such scales belong to, so they take three bf16 planes without
+// any, v = p0 + p1 + p2 with 24 significand bits, and the six products with i + j <= 2.  A value that is not finite is carried
+// by the first plane alone.
+constexpr float kLargest = 3.402823466e38f;
+__device__ __forceinline__ void split2(float v, uint16_t* h) {
+  const __half a = __float2half_rn(v);
+  float r = v - __half2float(a);
+  if (!(fabsf(r) <= kLargest)) r = 0.f;
+  h[0] = bits(a);
+  h[1] = bits(__float2half_rn(r));
+}
 __device__ __forceinline__ void split3(float v, uint16_t* p) {
   const __nv_bfloat16 a = __float2bfloat16_rn(v);
   float r = v - __bfloat162float(a);
-  if (!(fabsf(r) <= 3.402823466e38f)) r = 0.f;
+  if (!(fabsf(r) <= kLargest)) r = 0.f;
   const __nv_bfloat16 b = __float2bfloat16_rn(r);
   r -= __bfloat162float(b);
   p[0] = bits(a);
@@ -96,44 +108,87 @@ __device__ __forceinline__ void split3(float v, uint16_t* p) {
   p[2] = bits(__float2bfloat16_rn(r));
 }
 
-// Eight columns of a row of X or W as operand planes; what lies behind column d is zero.
+// Eight columns of a row; zero behind the last.
 template <typename T>
-__device__ __forceinline__ void pack8(const T* src, int64_t left, uint16_t* dst, int64_t plane) {
-  alignas(16) T v[8];
+__device__ __forceinline__ void load8(const T* src, int64_t left, T* v) {
   if (left >= 8 && ((uintptr_t)src & 15) == 0) {
 #pragma unroll
     for (int q = 0; q < (int)sizeof(T) / 2; ++q) reinterpret_cast<uint4*>(v)[q] = __ldg(reinterpret_cast<const uint4*>(src) + q);
   } else {
-    memset(v, 0, sizeof(v));
+    memset(v, 0, 8 * sizeof(T));
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (j < left) v[j] = src[j];
   }
-  if (sizeof(T) == 4) {
-    alignas(16) uint16_t w[3][8];
+}
+
+// Where a row's planes go: `scaled` two f16 planes and the row's factor 2^-e, `plain` three bf16 planes (float32), or
+// `plain` alone, the row as it is (16-bit types).  Null: not wanted.
+struct Planes {
+  uint16_t *plain, *scaled;
+  float* factor;
+  int64_t stride;  // elements from one plane to the next
+};
+
+// A warp packs a row of float32 (source null: a row of zeros).
+__device__ __forceinline__ void pack_row(const float* src, int64_t d, int64_t dp, const Planes& o, int64_t row) {
+  const int lane = threadIdx.x & 31;
+  float top = 0.f;
+  if (src)
+#pragma unroll 2
+    for (int64_t c = lane * 8; c < d; c += 256) {
+      alignas(16) float v[8];
+      load8(src + c, d - c, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float a = fabsf(v[j]);
+        if (a <= kLargest) top = fmaxf(top, a);
+      }
+    }
+  for (int q = 16; q; q >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, q));
+  int e = 0;
+  if (top > 0.f) {
+    frexpf(top, &e);
+    e = 15 - e;
+  }
+  e = min(e, 126);  // (the smallest e is -113; both 2^e and 2^-e are normal numbers)
+  const float scale = ldexpf(1.f, e);
+  if (lane == 0) o.factor[row] = ldexpf(1.f, -e);
+#pragma unroll 2
+  for (int64_t c = lane * 8; c < dp; c += 256) {
+    alignas(16) float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (src) load8(src + c, d - c, v);
+    alignas(16) uint16_t h[2][8], p[3][8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      uint16_t p[3];
-      split3(to_float(v[j]), p);
-      w[0][j] = p[0]; w[1][j] = p[1]; w[2][j] = p[2];
+      uint16_t q[3];
+      split2(v[j] * scale, q);
+      h[0][j] = q[0]; h[1][j] = q[1];
+      split3(v[j], q);
+      p[0][j] = q[0]; p[1][j] = q[1]; p[2][j] = q[2];
     }
 #pragma unroll
-    for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4*>(dst + p * plane) = *reinterpret_cast<uint4*>(w[p]);
-  } else {
-    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(v);
+    for (int k = 0; k < 2; ++k) *reinterpret_cast<uint4*>(o.scaled + k * o.stride + row * dp + c) = *reinterpret_cast<uint4*>(h[k]);
+    if (o.plain)
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(o.plain + k * o.stride + row * dp + c) = *reinterpret_cast<uint4*>(p[k]);
   }
 }
 
-// Entries of W as operand planes [planes][rows][dp], dp = d rounded up to 8.
-template <typename T>
-__global__ void __launch_bounds__(256) pack_kernel(const T* in, int64_t ld, int64_t rows, int64_t d, int64_t dp,
-                                                   uint16_t* out, int64_t plane) {
+// Entries of W as operand planes of [rows][dp], dp = d rounded up to 8.
+__global__ void __launch_bounds__(256) pack_rows_kernel(const float* in, int64_t ld, int64_t rows, int64_t d, int64_t dp, Planes o) {
+  pdl_sync();
+  for (int64_t r = blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8) pack_row(in + r * ld, d, dp, o, r);
+}
+__global__ void __launch_bounds__(256) pack_kernel(const __half* in, int64_t ld, int64_t rows, int64_t d, int64_t dp, Planes o) {
   pdl_sync();
   // a piece has fewer than 2^31 groups of eight (it is 256 MiB, or 4096 entries of at most 2^20 columns)
   const uint32_t per_row = (uint32_t)(dp / 8), total = (uint32_t)rows * per_row;
   for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < total; i += gridDim.x * blockDim.x) {
     const int64_t r = i / per_row, c = (i % per_row) * 8;
-    pack8(in + r * ld + c, d - c, out + r * dp + c, plane);
+    alignas(16) __half v[8];
+    load8(in + r * ld + c, d - c, v);
+    *reinterpret_cast<uint4*>(o.plain + r * dp + c) = *reinterpret_cast<uint4*>(v);
   }
 }
 
@@ -145,8 +200,7 @@ constexpr int kRowThreads = 512;
 template <typename T, typename Index>
 __global__ void __launch_bounds__(kRowThreads) rows_kernel(const Index* target, int64_t n, int64_t v, int64_t ignore,
                                                            const float* g, int64_t g_stride, const float* lse, Rows r,
-                                                           const T* x, int64_t ld, int64_t d, int64_t dp, uint16_t* out,
-                                                           int64_t plane) {
+                                                           const T* x, int64_t ld, int64_t d, int64_t dp, Planes o) {
   __shared__ int before_of[kRowThreads / 32], all_of[kRowThreads / 32];
   __shared__ float top_of[kRowThreads / 32];
   __shared__ int list[kRowThreads];
@@ -217,31 +271,54 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const Index* target, 
       }
     }
     __syncthreads();
-    for (uint32_t k = threadIdx.x; k < (uint32_t)count * per_row; k += kRowThreads) {
-      const uint32_t j = k / per_row;
-      const int64_t c = (k % per_row) * 8;
-      pack8(x + (base + list[j]) * ld + c, d - c, out + (before + j) * dp + c, plane);
+    if constexpr (sizeof(T) == 4) {
+      for (int j = warp; j < count; j += kRowThreads / 32) pack_row(x + (base + list[j]) * ld, d, dp, o, before + j);
+    } else {
+      for (uint32_t k = threadIdx.x; k < (uint32_t)count * per_row; k += kRowThreads) {
+        const uint32_t j = k / per_row;
+        const int64_t c = (k % per_row) * 8;
+        alignas(16) T v[8];
+        load8(x + (base + list[j]) * ld + c, d - c, v);
+        *reinterpret_cast<uint4*>(o.plain + (before + j) * dp + c) = *reinterpret_cast<uint4*>(v);
+      }
     }
     before += count;
   }
   const int64_t end = (all + (int64_t)kTile - 1) / kTile * kTile;
-  for (int64_t k = blockIdx.x * (int64_t)kRowThreads + threadIdx.x; k < (end - all) * per_row; k += (int64_t)gridDim.x * kRowThreads)
-#pragma unroll
-    for (int p = 0; p < (sizeof(T) == 4 ? 3 : 1); ++p)
-      *reinterpret_cast<uint4*>(out + p * plane + all * dp + k * 8) = make_uint4(0, 0, 0, 0);
+  if constexpr (sizeof(T) == 4) {
+    for (int64_t r = all + blockIdx.x * (kRowThreads / 32) + warp; r < end; r += gridDim.x * (kRowThreads / 32))
+      pack_row(nullptr, d, dp, o, r);
+  } else {
+    for (int64_t k = blockIdx.x * (int64_t)kRowThreads + threadIdx.x; k < (end - all) * per_row; k += (int64_t)gridDim.x * kRowThreads)
+      *reinterpret_cast<uint4*>(o.plain + all * dp + k * 8) = make_uint4(0, 0, 0, 0);
+  }
 }
 
 // ---- epilogues ------------------------------------------------------------------------------------------------------
+// float32 operands are scaled by row (pack_row): the logits of a thread's row and columns, unscaled.
+template <int C>
+__device__ __forceinline__ void unscale(float (&acc)[C], const float* row_factor, const float* col_factor, int row, int col0) {
+  const float f = row_factor[row];
+#pragma unroll
+  for (int j = 0; j < C; j += 4) {
+    const float4 q = __ldg(reinterpret_cast<const float4*>(col_factor + col0 + j));
+    acc[j] *= f * q.x; acc[j + 1] *= f * q.y; acc[j + 2] *= f * q.z; acc[j + 3] *= f * q.w;
+  }
+}
+
 // Forward: maximum and sum of exp(z - maximum) over this thread's columns, and the target's logit.
+template <bool F32>
 struct ForwardEpi {
   const Head* head;
   const int* target;
   float2* part;      // [parts][n_pad]
   float* hit;        // [n_pad] the target's logit
   int64_t n_pad, v0, v, part0;  // first vocabulary entry of this launch, entries of it; number of its first part
+  const float *row_factor, *col_factor;
   template <int C>
   __device__ void operator()(float (&acc)[C], int row, int col0, int, const CUtensorMap*, const pg::Out&) const {
     if (row >= head->live || col0 >= v) return;
+    if (F32) unscale(acc, row_factor, col_factor, row, col0);
     const int have = (int)min(v - col0, (int64_t)C);
     const int64_t at = (int64_t)target[row] - v0 - col0;
     const int t = at >= 0 && at < have ? (int)at : -1;
@@ -316,10 +393,12 @@ struct GradEpi {
   const float* share;
   const float* lse;
   int64_t ld, v0, v;
+  const float *row_factor, *col_factor;
   template <int C>
   __device__ void operator()(float (&acc)[C], int row, int col0, int, const CUtensorMap* tm, const pg::Out& out) const {
     if (col0 >= ld) return;
     const bool live = row < head->live;
+    if (TYPE == kF32 && live) unscale(acc, row_factor, col_factor, row, col0);
     const float g = live ? share[row] : 0.f, l = live ? lse[row] : 0.f;
     const int64_t at = live ? (int64_t)target[row] - v0 - col0 : -1;
     const int t = at >= 0 && at < C ? (int)at : -1;
@@ -472,7 +551,8 @@ struct Layout {
   bool few_fwd, few_bwd;         // the kernels for few rows: nothing is packed, no dZ is kept
   int64_t fwd_bytes, bwd_bytes;
   // byte offsets
-  int64_t place, target, share, lse, hit, part, x, w_fwd, w_bwd, dz, sums;
+  int64_t place, target, share, lse, hit, part, x, x_scaled, x_factor, w_fwd, w_fwd_factor, w_bwd, w_bwd_scaled, w_bwd_factor, dz,
+      sums;
 };
 
 bool pack_w(const tcb200_linear_ce_t& p) { return p.dtype == TCB200_F32 || p.pack_w; }
@@ -496,11 +576,12 @@ int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
     const int64_t pieces = ceil_div(v_pad, most);
     return round_up(ceil_div(v_pad, pieces), kTile);
   };
-  l->fwd_piece = pack_w(p) ? piece(l->dp * 2 * l->planes) : v_pad;
+  l->fwd_piece = pack_w(p) ? piece(l->dp * 2 * std::min<int64_t>(l->planes, 2)) : v_pad;
   l->bwd_piece = piece(2 * l->planes * (pack_w(p) ? std::max(l->dp, l->n_pad) : l->n_pad));
-  const int products = l->planes == 3 ? 6 : 1;
-  l->fwd_bn = pg::tile_columns(l->n_pad, l->fwd_piece, p.D, products, sms);
-  l->bwd_bn = pg::tile_columns(l->n_pad, l->bwd_piece, p.D, products, sms);
+  const bool f32 = p.dtype == TCB200_F32;
+  const int products = f32 ? 6 : 1, z_products = f32 ? 3 : 1;
+  l->fwd_bn = pg::tile_columns(l->n_pad, l->fwd_piece, p.D, z_products, sms);
+  l->bwd_bn = pg::tile_columns(l->n_pad, l->bwd_piece, p.D, z_products, sms);
   l->dw_bn = pg::tile_columns(l->bwd_piece, p.D, p.N, products, sms);
   l->few_fwd = few_forward_ok(p);
   l->few_bwd = few_backward_ok(p);
@@ -531,14 +612,25 @@ int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
   l->target = take(l->n_pad * 4);
   l->share = take(l->n_pad * 4);
   l->lse = take(l->n_pad * 4);
-  l->x = take(l->few_fwd && l->few_bwd ? 0 : l->planes * l->n_pad * l->dp * 2);
+  // X: the plain planes, unless float32 goes forward, and the scaled ones of float32
+  const int64_t x_plane = l->few_fwd && l->few_bwd ? 0 : l->n_pad * l->dp * 2;
+  l->x_factor = take(f32 ? l->n_pad * 4 : 0);
+  l->x_scaled = take(f32 ? 2 * x_plane : 0);
+  l->x = f32 ? -1 : take(x_plane);
   const int64_t common = at;
   l->hit = take(l->n_pad * 4);
   l->part = take(l->parts * l->n_pad * 8);
-  l->w_fwd = take(pack_w(p) && !l->few_fwd ? l->planes * l->fwd_piece * l->dp * 2 : 0);
+  // W: one packed piece
+  const int64_t fwd_plane = pack_w(p) && !l->few_fwd ? l->fwd_piece * l->dp * 2 : 0;
+  l->w_fwd = take(f32 ? 2 * fwd_plane : fwd_plane);
+  l->w_fwd_factor = take(f32 ? l->fwd_piece * 4 : 0);
   l->fwd_bytes = at;
   at = common;
-  l->w_bwd = take(pack_w(p) && !l->few_bwd ? l->planes * l->bwd_piece * l->dp * 2 : 0);
+  if (f32) l->x = take(3 * x_plane);
+  const int64_t bwd_plane = pack_w(p) && !l->few_bwd ? l->bwd_piece * l->dp * 2 : 0;
+  l->w_bwd = take(l->planes * bwd_plane);
+  l->w_bwd_scaled = take(f32 ? 2 * bwd_plane : 0);
+  l->w_bwd_factor = take(f32 ? l->bwd_piece * 4 : 0);
   l->dz = take(l->few_bwd ? 0 : l->planes * l->n_pad * l->bwd_piece * 2);
   l->sum_rows = l->few_bwd ? kFewRows : l->n_pad;
   l->sums = take((int64_t)l->splits * l->sum_rows * l->dp * 4);
@@ -558,65 +650,68 @@ Rows rows_of(char* ws, const Layout& l) {
 
 template <typename T, typename Index>
 int launch_rows_typed(const tcb200_linear_ce_t& p, const Layout& l, const void* X, const void* target, const float* g,
-                      int64_t g_stride, const float* lse, const Rows& r, void* out, int sms, cudaStream_t s) {
+                      int64_t g_stride, const float* lse, const Rows& r, const Planes& o, int sms, cudaStream_t s) {
   // blocks enough for the rows' copies, zero rows of the last tile among them
   const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(l.n_pad * (l.dp / 8), kRowThreads), 2ll * sms);
   TCB200_CUDA_TRY(launch_pdl(rows_kernel<T, Index>, dim3(blocks), dim3(kRowThreads), 0, s, static_cast<const Index*>(target),
-                             p.N, p.V, p.ignore_index, g, g_stride, lse, r, static_cast<const T*>(X), p.ldx, p.D, l.dp,
-                             static_cast<uint16_t*>(out), l.n_pad * l.dp));
+                             p.N, p.V, p.ignore_index, g, g_stride, lse, r, static_cast<const T*>(X), p.ldx, p.D, l.dp, o));
   return TCB200_OK;
 }
 // f16 and bf16 are copied as they are
 int launch_rows(const tcb200_linear_ce_t& p, const Layout& l, const void* X, const void* target, const float* g,
-                int64_t g_stride, const float* lse, const Rows& r, void* out, int sms, cudaStream_t s) {
+                int64_t g_stride, const float* lse, const Rows& r, char* ws, int sms, cudaStream_t s) {
+  Planes o{l.x < 0 || (p.dtype == TCB200_F32 && !g) ? nullptr : reinterpret_cast<uint16_t*>(ws + l.x), reinterpret_cast<uint16_t*>(ws + l.x_scaled),
+           reinterpret_cast<float*>(ws + l.x_factor), l.n_pad * l.dp};
   const bool f32 = p.dtype == TCB200_F32, wide = p.index_bytes == 8;
   auto fn = f32 ? (wide ? launch_rows_typed<float, int64_t> : launch_rows_typed<float, int32_t>)
                 : (wide ? launch_rows_typed<__half, int64_t> : launch_rows_typed<__half, int32_t>);
-  return fn(p, l, X, target, g, g_stride, lse, r, out, sms, s);
+  return fn(p, l, X, target, g, g_stride, lse, r, o, sms, s);
 }
 
-int launch_pack(const tcb200_linear_ce_t& p, const Layout& l, const void* in, int64_t rows, void* out, int64_t plane, int sms,
-                cudaStream_t s) {
-  const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows * (l.dp / 8), 256), 8ll * sms)));
-  uint16_t* o = static_cast<uint16_t*>(out);
-  if (p.dtype == TCB200_F32)
-    TCB200_CUDA_TRY(launch_pdl(pack_kernel<float>, grid, dim3(256), 0, s, static_cast<const float*>(in), p.ldw, rows, p.D, l.dp, o, plane));
-  else
-    TCB200_CUDA_TRY(launch_pdl(pack_kernel<__half>, grid, dim3(256), 0, s, static_cast<const __half*>(in), p.ldw, rows, p.D, l.dp, o, plane));
+int launch_pack(const tcb200_linear_ce_t& p, const Layout& l, const void* in, int64_t rows, const Planes& o, int sms, cudaStream_t s) {
+  if (p.dtype == TCB200_F32) {
+    const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, 8), 8ll * sms)));
+    TCB200_CUDA_TRY(launch_pdl(pack_rows_kernel, grid, dim3(256), 0, s, static_cast<const float*>(in), p.ldw, rows, p.D, l.dp, o));
+  } else {
+    const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows * (l.dp / 8), 256), 8ll * sms)));
+    TCB200_CUDA_TRY(launch_pdl(pack_kernel, grid, dim3(256), 0, s, static_cast<const __half*>(in), p.ldw, rows, p.D, l.dp, o));
+  }
   return TCB200_OK;
 }
 
 size_t elem_bytes(const tcb200_linear_ce_t& p) { return p.dtype == TCB200_F32 ? 4 : 2; }
 
-// `forward`: the loss keeps fp32 accuracy whatever the inputs' type.
-pg::Args gemm_args(const Layout& l, int64_t M, int64_t N, int64_t K, const int* live, int live_is_k, int* status, bool forward) {
+// `products`: plane products per k-block.  `forward`: the loss keeps fp32 accuracy whatever the inputs' type.
+pg::Args gemm_args(int64_t M, int64_t N, int64_t K, const int* live, int live_is_k, int* status, int products, bool forward) {
   pg::Args a = {};
   a.M = M;
   a.N = N;
   a.K = K;
   a.live = live;
   a.live_is_k = live_is_k;
-  a.products = l.planes == 3 ? 6 : 1;
-  // A drain every 512 k (32 MMAs), 256 k of float32 operands (16 MMAs of the largest planes after 80 of smaller ones): the
+  a.products = products;
+  // A drain every 512 k (32 MMAs), 256 k of float32 operands (16 MMAs of the largest planes after those of smaller ones): the
   // truncation of the tensor core's sums then stays near 2^-20 of a term's size.  Gradients that are rounded to 16 bits
   // in the end take 1024 k: half as many drains, which leaves the epilogues twice the time before they hold up the MMAs
   // (dZ of 4096 x 2048 x 32000: 414 -> 350 us).
-  a.chunk_kb = l.planes == 3 ? 4 : forward ? 8 : 16;
+  a.chunk_kb = products > 1 ? 4 : forward ? 8 : 16;
   a.splits = 1;
   a.dev_status = status;
   return a;
 }
 
-// The operand of entries [v0, v0 + v) of W: in place, or packed into `packed`.
-int w_operand(const tcb200_linear_ce_t& p, const Layout& l, const void* W, int64_t v0, int64_t v, int64_t piece, void* packed,
-              int sms, cudaStream_t s, pg::Operand* o) {
+// The operands of entries [v0, v0 + v) of W: in place, or packed into `o` (rows of dp).  `z` is the logits' operand, `plain` the
+// gradient's.
+int w_operands(const tcb200_linear_ce_t& p, const Layout& l, const void* W, int64_t v0, int64_t v, const Planes& o, int sms,
+               cudaStream_t s, pg::Operand* z, pg::Operand* plain) {
   const char* base = static_cast<const char*>(W) + (size_t)v0 * p.ldw * elem_bytes(p);
   if (!pack_w(p)) {
-    *o = {base, p.D, v, p.ldw, 1, 0};
+    *z = *plain = {base, p.D, v, p.ldw, 1, 0};
     return TCB200_OK;
   }
-  *o = {packed, l.dp, v, l.dp, l.planes, piece * l.dp};
-  return launch_pack(p, l, base, v, packed, piece * l.dp, sms, s);
+  *plain = {o.plain, l.dp, v, l.dp, l.planes, o.stride};
+  *z = p.dtype == TCB200_F32 ? pg::Operand{o.scaled, l.dp, v, l.dp, 2, o.stride} : *plain;
+  return launch_pack(p, l, base, v, o, sms, s);
 }
 
 int current_device(int* device) {
@@ -627,27 +722,33 @@ int current_device(int* device) {
 template <typename T, int TYPE>
 int backward_typed(const tcb200_linear_ce_t& p, const Layout& l, const void* W, const Rows& r, char* ws, T* dX, T* dW,
                    int device, int sms, cudaStream_t s, int* status, int* dev_status) {
-  const bool bf16 = TYPE != kF16;
+  const bool bf16 = TYPE != kF16, f32 = TYPE == kF32;
   const float scale = TYPE == kF16 ? 1.f / kHalfScale : 1.f;
+  const int products = f32 ? 6 : 1;
   const pg::Operand x{ws + l.x, l.dp, l.n_pad, l.dp, l.planes, l.n_pad * l.dp};
+  const pg::Operand zx = f32 ? pg::Operand{ws + l.x_scaled, l.dp, l.n_pad, l.dp, 2, l.n_pad * l.dp} : x;
+  const Planes packed{reinterpret_cast<uint16_t*>(ws + l.w_bwd), reinterpret_cast<uint16_t*>(ws + l.w_bwd_scaled),
+                      reinterpret_cast<float*>(ws + l.w_bwd_factor), l.bwd_piece * l.dp};
   float* sums = reinterpret_cast<float*>(ws + l.sums);
+  const int* live = &r.head->live;
   int st;
   for (int64_t v0 = 0; v0 < p.V; v0 += l.bwd_piece) {
     const int64_t v = std::min(l.bwd_piece, p.V - v0), ld = l.bwd_piece;
-    pg::Operand w;
-    if ((st = w_operand(p, l, W, v0, v, l.bwd_piece, ws + l.w_bwd, sms, s, &w)) != TCB200_OK) return st;
+    pg::Operand zw, w;
+    if ((st = w_operands(p, l, W, v0, v, packed, sms, s, &zw, &w)) != TCB200_OK) return st;
     uint16_t* dz = reinterpret_cast<uint16_t*>(ws + l.dz);
-    const GradEpi<TYPE> ge{r.head, r.target, r.share, r.lse, ld, v0, v};
+    const GradEpi<TYPE> ge{r.head, r.target, r.share, r.lse, ld, v0, v, reinterpret_cast<const float*>(ws + l.x_factor), packed.factor};
     CUtensorMap tc;
     if ((st = pg::make_out_map(&tc, {dz, ld, l.n_pad, ld, l.planes, l.n_pad * ld}, 2)) != TCB200_OK) return st;
-    st = pg::launch_columns<false, false>(l.bwd_bn, x, w, bf16, gemm_args(l, p.N, v, p.D, &r.head->live, 0, status, false), tc, ge, device, sms, s);
+    st = pg::launch_columns<false, false>(l.bwd_bn, zx, zw, TYPE == kBF16, gemm_args(p.N, v, p.D, live, 0, status, f32 ? 3 : 1, false), tc,
+                                          ge, device, sms, s);
     if (st != TCB200_OK) return st;
     const pg::Operand z{dz, v, l.n_pad, ld, l.planes, l.n_pad * ld};
     if (dX) {
       const SumEpi se{l.dp, v0 > 0};
       st = pg::make_out_map(&tc, {sums, l.dp, l.n_pad, l.dp, l.splits, l.n_pad * l.dp}, 4);
       if (st != TCB200_OK) return st;
-      pg::Args a = gemm_args(l, p.N, p.D, v, &r.head->live, 0, status, false);
+      pg::Args a = gemm_args(p.N, p.D, v, live, 0, status, products, false);
       a.splits = l.splits;
       a.split_kb = (int)ceil_div(ceil_div(v, pg::kBK), l.splits);
       if ((st = pg::launch<256, false, true>(z, w, bf16, a, tc, se, device, sms, s)) != TCB200_OK) return st;
@@ -657,7 +758,8 @@ int backward_typed(const tcb200_linear_ce_t& p, const Layout& l, const void* W, 
       const int tma = (p.D * sizeof(T)) % 16 == 0 && ((uintptr_t)out & 15) == 0;
       if (tma && (st = pg::make_out_map(&tc, {out, p.D, v, p.D, 1, 0}, sizeof(T))) != TCB200_OK) return st;
       const WeightEpi<T> we{r.head, out, v, p.D, scale, tma};
-      st = pg::launch_columns<true, true>(l.dw_bn, z, x, bf16, gemm_args(l, v, p.D, p.N, &r.head->live, 1, status, false), tc, we, device, sms, s);
+      st = pg::launch_columns<true, true>(l.dw_bn, z, x, bf16, gemm_args(v, p.D, p.N, live, 1, status, products, false), tc, we, device,
+                                          sms, s);
       if (st != TCB200_OK) return st;
     }
   }
@@ -703,16 +805,25 @@ int tcb200_linear_ce_forward(const tcb200_linear_ce_t* problem, const void* X, c
   float2* part = reinterpret_cast<float2*>(ws + l.part);
   float* hit = reinterpret_cast<float*>(ws + l.hit);
   st = l.few_fwd ? few_forward(p, X, W, target, r, part, hit, l.n_pad, device, sms, s)
-                 : launch_rows(p, l, X, target, nullptr, 0, nullptr, r, ws + l.x, sms, s);
+                 : launch_rows(p, l, X, target, nullptr, 0, nullptr, r, ws, sms, s);
   if (st != TCB200_OK) return st;
-  const pg::Operand x{ws + l.x, l.dp, l.n_pad, l.dp, l.planes, l.n_pad * l.dp};
+  const bool f32 = p.dtype == TCB200_F32;
+  const pg::Operand x = f32 ? pg::Operand{ws + l.x_scaled, l.dp, l.n_pad, l.dp, 2, l.n_pad * l.dp}
+                            : pg::Operand{ws + l.x, l.dp, l.n_pad, l.dp, 1, 0};
+  uint16_t* packed = reinterpret_cast<uint16_t*>(ws + l.w_fwd);
+  const Planes o{f32 ? nullptr : packed, f32 ? packed : nullptr, reinterpret_cast<float*>(ws + l.w_fwd_factor), l.fwd_piece * l.dp};
   for (int64_t v0 = l.few_fwd ? p.V : 0; v0 < p.V; v0 += l.fwd_piece) {
-    const int64_t v = std::min(l.fwd_piece, p.V - v0);
-    pg::Operand w;
-    if ((st = w_operand(p, l, W, v0, v, l.fwd_piece, ws + l.w_fwd, sms, s, &w)) != TCB200_OK) return st;
-    const ForwardEpi e{r.head, r.target, part, hit, l.n_pad, v0, v, v0 / (l.fwd_bn / 2)};
-    st = pg::launch_columns<false, false>(l.fwd_bn, x, w, p.dtype != TCB200_F16, gemm_args(l, p.N, v, p.D, &r.head->live, 0, status, true),
-                                  CUtensorMap{}, e, device, sms, s);
+    const int64_t v = std::min(l.fwd_piece, p.V - v0), part0 = v0 / (l.fwd_bn / 2);
+    pg::Operand w, unused;
+    if ((st = w_operands(p, l, W, v0, v, o, sms, s, &w, &unused)) != TCB200_OK) return st;
+    const pg::Args args = gemm_args(p.N, v, p.D, &r.head->live, 0, status, f32 ? 3 : 1, true);
+    if (f32) {
+      const ForwardEpi<true> e{r.head, r.target, part, hit, l.n_pad, v0, v, part0, reinterpret_cast<const float*>(ws + l.x_factor), o.factor};
+      st = pg::launch_columns<false, false>(l.fwd_bn, x, w, false, args, CUtensorMap{}, e, device, sms, s);
+    } else {
+      const ForwardEpi<false> e{r.head, r.target, part, hit, l.n_pad, v0, v, part0, nullptr, nullptr};
+      st = pg::launch_columns<false, false>(l.fwd_bn, x, w, p.dtype == TCB200_BF16, args, CUtensorMap{}, e, device, sms, s);
+    }
     if (st != TCB200_OK) return st;
   }
   TCB200_CUDA_TRY(launch_pdl(join_kernel, dim3((unsigned)ceil_div(p.N, 32)), dim3(32, 32), 0, s, r,
@@ -745,7 +856,7 @@ int tcb200_linear_ce_backward(const tcb200_linear_ce_t* problem, const void* X, 
   if (l.few_bwd)
     return few_backward(p, X, W, target, lse, grad_loss, grad_stride, r, reinterpret_cast<float*>(ws + l.sums),
                         l.sum_rows * l.dp, l.dp, dX, dW, device, sms, s);
-  st = launch_rows(p, l, X, target, grad_loss, grad_stride, lse, r, ws + l.x, sms, s);
+  st = launch_rows(p, l, X, target, grad_loss, grad_stride, lse, r, ws, sms, s);
   if (st != TCB200_OK) return st;
   switch (p.dtype) {
     case TCB200_F32:

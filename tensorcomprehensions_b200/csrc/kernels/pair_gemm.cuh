@@ -4,8 +4,9 @@
 //
 // Operands are f16 or bf16 (both the same), each either k-major (rows of k) or mn-major (rows of m or n): the three
 // products of a linear layer's training step (X W^T, dZ W, dZ^T X) then read the same arrays without a transposed copy.
-// float32 operands arrive as three bf16 planes a = a0 + a1 + a2 (8 + 8 + 8 significand bits); of the nine plane products
-// the six with i + j <= 2 are summed, smallest first, and the largest dropped one is 2^-24 of the product.
+// float32 operands arrive as two f16 planes (11 + 11 significand bits, scaled) or three bf16 planes (8 + 8 + 8); of the plane
+// products those with i + j <= 1, or <= 2, are summed, smallest first: the largest dropped one is 2^-22, or 2^-24, of the
+// product at most.
 //
 // Roles of a CTA: warps 0-7 drain the accumulator and run the epilogue, warp 8 issues the TMA loads of this CTA's
 // 128 rows of A and BN / 2 of the tile's BN rows of B, the leader's warp 9 issues the MMAs (M = 256, N = BN, K = 16) of both
@@ -45,7 +46,7 @@ struct Args {
   int64_t M, N, K;          // extents; one of them may be replaced by *live
   const int* live;          // null, or a device count that replaces M (live_is_k = 0) or K (live_is_k = 1)
   int live_is_k;
-  int products;             // plane products per k-block: 1, or 6 for float32
+  int products;             // plane products per k-block: 1, or 3 or 6 for float32
   int pa[kMaxProducts], pb[kMaxProducts];
   int chunk_kb;             // k-blocks per drain
   int splits, split_kb;     // the reduction's k-blocks go to `splits` units of split_kb each
@@ -378,10 +379,11 @@ int launch(const Operand& A, const Operand& B, bool bf16, Args args, const CUten
   if (st == TCB200_OK) st = make_map(&tb, B, bf16, B_MN, BN / 2);
   if (st != TCB200_OK) return st;
   args.idesc = make_idesc(bf16, A_MN, B_MN, BN);
-  if (args.products == 1) args.pa[0] = args.pb[0] = 0;
-  else {
-    const int pa[6] = {2, 1, 0, 1, 0, 0}, pb[6] = {0, 1, 2, 0, 1, 0};
-    for (int i = 0; i < 6; ++i) args.pa[i] = pa[i], args.pb[i] = pb[i];
+  // the planes of each product, smallest products first: of one plane, of two (i + j <= 1) or of three (i + j <= 2)
+  static const int pa[6] = {2, 1, 0, 1, 0, 0}, pb[6] = {0, 1, 2, 0, 1, 0};
+  for (int i = 0; i < args.products; ++i) {
+    args.pa[i] = pa[6 - args.products + i];
+    args.pb[i] = pb[6 - args.products + i];
   }
   const int64_t units = ceil_div(args.M, kTile) * ceil_div(args.N, BN) * args.splits;
   if (units == 0) return TCB200_OK;
