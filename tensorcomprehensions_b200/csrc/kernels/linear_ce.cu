@@ -274,12 +274,22 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const Index* target, 
     if constexpr (sizeof(T) == 4) {
       for (int j = warp; j < count; j += kRowThreads / 32) pack_row(x + (base + list[j]) * ld, d, dp, o, before + j);
     } else {
-      for (uint32_t k = threadIdx.x; k < (uint32_t)count * per_row; k += kRowThreads) {
-        const uint32_t j = k / per_row;
-        const int64_t c = (k % per_row) * 8;
-        alignas(16) T v[8];
-        load8(x + (base + list[j]) * ld + c, d - c, v);
-        *reinterpret_cast<uint4*>(o.plain + (before + j) * dp + c) = *reinterpret_cast<uint4*>(v);
+      const uint32_t items = (uint32_t)count * per_row;
+      constexpr int U = 4;  // loads in flight a thread
+      for (uint32_t k0 = threadIdx.x; k0 < items; k0 += U * kRowThreads) {
+        alignas(16) T v[U][8];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const uint32_t k = k0 + u * kRowThreads, j = k / per_row;
+          const int64_t c = (k % per_row) * 8;
+          if (k < items) load8(x + (base + list[j]) * ld + c, d - c, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const uint32_t k = k0 + u * kRowThreads, j = k / per_row;
+          const int64_t c = (k % per_row) * 8;
+          if (k < items) *reinterpret_cast<uint4*>(o.plain + (before + j) * dp + c) = *reinterpret_cast<uint4*>(v[u]);
+        }
       }
     }
     before += count;
@@ -309,6 +319,7 @@ __device__ __forceinline__ void unscale(float (&acc)[C], const float* row_factor
 // Forward: maximum and sum of exp(z - maximum) over this thread's columns, and the target's logit.
 template <bool F32>
 struct ForwardEpi {
+  static constexpr int kColumns = 128;
   const Head* head;
   const int* target;
   float2* part;      // [parts][n_pad]
@@ -388,6 +399,9 @@ enum { kF32 = 0, kF16 = 1, kBF16 = 2 };
 
 template <int TYPE>
 struct GradEpi {
+  // three planes of a float32 value are five times the work of one rounding: sixteen warps of 64 columns
+  // (1024 x 1024 x 16384: 120 -> 102 us), where 16-bit types lose by them (4096 x 2048 x 32000: 348 -> 361 us)
+  static constexpr int kColumns = TYPE == kF32 ? 64 : 128;
   const Head* head;
   const int* target;
   const float* share;
@@ -439,6 +453,7 @@ struct GradEpi {
 
 // dX of a piece: fp32 sums, one plane per split of the piece, added to over the pieces.
 struct SumEpi {
+  static constexpr int kColumns = 128;
   int64_t ld;  // columns of the sums
   int add;
   template <int C>
@@ -460,6 +475,7 @@ struct SumEpi {
 // dW of a piece: whole sums, scaled and rounded once.
 template <typename T>
 struct WeightEpi {
+  static constexpr int kColumns = 128;
   const Head* head;
   T* dst;
   int64_t rows, d;

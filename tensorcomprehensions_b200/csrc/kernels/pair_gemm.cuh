@@ -1,6 +1,6 @@
 // 16-bit matrix products on CTA pairs with fp32 accuracy of the sum, shared by the kernels of the large-vocabulary
 // losses (sm_100a).  One pair computes a tile C(m, n) = sum_k A(m, k) B(n, k) of 256 rows and BN = 256 or 128 columns; the
-// epilogue is a functor that gets a row and BN / 2 consecutive columns of it in registers.
+// epilogue is a functor that gets a row and C consecutive columns of it in registers.
 //
 // Operands are f16 or bf16 (both the same), each either k-major (rows of k) or mn-major (rows of m or n): the three
 // products of a linear layer's training step (X W^T, dZ W, dZ^T X) then read the same arrays without a transposed copy.
@@ -8,9 +8,8 @@
 // products those with i + j <= 1, or <= 2, are summed, smallest first: the largest dropped one is 2^-22, or 2^-24, of the
 // product at most.
 //
-// Roles of a CTA: warps 0-7 drain the accumulator and run the epilogue, warp 8 issues the TMA loads of this CTA's
-// 128 rows of A and BN / 2 of the tile's BN rows of B, the leader's warp 9 issues the MMAs (M = 256, N = BN, K = 16) of both
-// CTAs.  In both issuing warps all lanes run the loop and one elected lane issues, so that descriptors and addresses stay in
+// Roles of a CTA: 4 BN / C warps drain the accumulator and run the epilogue, one issues the TMA loads of this CTA's 128 rows
+// of A and BN / 2 of the tile's BN rows of B, and the leader's last one issues the MMAs (M = 256, N = BN, K = 16) of both CTAs.  In both issuing warps all lanes run the loop and one elected lane issues, so that descriptors and addresses stay in
 // uniform registers.  With loops that only lane 0 ran, a k-block's loads took 400 cycles to issue and its four MMAs 300, and a
 // k-block 740 cycles where its MMAs take 512 (4096 x 2048 x 32000, forward: 393 us; now 332 us, 1.62 PFLOP/s).  Of the rest
 // two issuers with half of the columns each, shorter or longer rings (4 to 6 stages) and higher boxes gained nothing.
@@ -31,15 +30,16 @@ constexpr int kHalf = 128;      // rows of A, and of B at most, that one CTA loa
 constexpr int kBK = 64;         // k of a stage: one 128-byte swizzle row of 16-bit values
 constexpr int kOperandBytes = kHalf * kBK * 2;
 constexpr int kStageBytes = 2 * kOperandBytes;
-constexpr int kStages = 6;
-constexpr int kDrainWarps = 8;
-constexpr int kThreads = (kDrainWarps + 2) * 32;
+// BN: columns of a tile; C: columns of a drain warp (there are four lane quarters of tensor memory).
+__host__ __device__ constexpr int drain_warps(int bn, int c) { return 4 * (bn / c); }
+__host__ __device__ constexpr int block_threads(int bn, int c) { return (drain_warps(bn, c) + 2) * 32; }
+__host__ __device__ constexpr int stages(int bn, int c) { return drain_warps(bn, c) > 8 ? 5 : 6; }
 constexpr int kBarrierBytes = 256;
 constexpr int kOutBytes = 4096;  // staging of a drain warp: 32 rows of 128 bytes
-constexpr int kOutOffset = kStages * kStageBytes;
-constexpr int kBarrierOffset = kOutOffset + kDrainWarps * kOutBytes;
-constexpr int kSmemBytes = kBarrierOffset + kBarrierBytes + 1024;
-static_assert(kSmemBytes <= 227 * 1024, "the stages exceed shared memory");
+__host__ __device__ constexpr int out_offset(int bn, int c) { return stages(bn, c) * kStageBytes; }
+__host__ __device__ constexpr int barrier_offset(int bn, int c) { return out_offset(bn, c) + drain_warps(bn, c) * kOutBytes; }
+__host__ __device__ constexpr int smem_bytes(int bn, int c) { return barrier_offset(bn, c) + kBarrierBytes + 1024; }
+static_assert(smem_bytes(256, 128) <= 227 * 1024 && smem_bytes(256, 64) <= 227 * 1024, "the stages exceed shared memory");
 constexpr int kMaxProducts = 6;
 
 struct Args {
@@ -186,17 +186,18 @@ struct Out {
 };
 
 // Epi: struct with  template <int C> __device__ void operator()(float (&acc)[C], int row, int col0, int split,
-// const CUtensorMap* tm, const Out& out)  where row and col0 are the thread's row and first of its C = BN / 2 columns (both
+// const CUtensorMap* tm, const Out& out)  where row and col0 are the thread's row and first of its C columns (both
 // may lie outside the result).
-template <int BN, bool A_MN, bool B_MN, class Epi>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+template <int BN, int C, bool A_MN, bool B_MN, class Epi>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(block_threads(BN, C), 1)
 pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                  const __grid_constant__ CUtensorMap tmC, const __grid_constant__ Args a, const __grid_constant__ Epi epi) {
   static_assert(BN == 256 || BN == 128, "an operand's mn-major rows are whole 64-element groups in each CTA");
-  constexpr int C = BN / 2;  // columns of a drain warp; rows of B that this CTA loads
+  constexpr int B_ROWS = BN / 2;  // rows of B that this CTA loads
+  constexpr int DRAIN = drain_warps(BN, C), kStages = stages(BN, C);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kBarrierOffset);  // used in the leader: both CTAs' loads
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + barrier_offset(BN, C));  // used in the leader: both CTAs' loads
   uint64_t* empty = full + kStages;
   uint64_t* acc_full = empty + kStages;   // [2]
   uint64_t* acc_empty = acc_full + 2;     // [2], used in the leader: the drain warps of both CTAs
@@ -215,12 +216,12 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 2 * kDrainWarps);
+      mbar_init(&acc_empty[b], 2 * DRAIN);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kDrainWarps + 1) tmem_alloc_pair(tmem_slot, 512);
+  if (warp == DRAIN + 1) tmem_alloc_pair(tmem_slot, 512);
   tc_fence_before();
   cluster_sync_all();
   tc_fence_after();
@@ -229,7 +230,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 
   const Units units(a, BN);
 
-  if (warp == kDrainWarps) {
+  if (warp == DRAIN) {
     // ------------------------------------------------ TMA producer
     const bool issuer = elect_one();
     const uint32_t full0 = map_to_rank(&full[0], 0);
@@ -240,7 +241,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       int64_t tm, tn;
       int split, kb0, nkb;
       units.locate(u, &tm, &tn, &split, &kb0, &nkb);
-      const int m0 = (int)(tm * kTile) + (int)rank * kHalf, n0 = (int)(tn * BN) + (int)rank * C;
+      const int m0 = (int)(tm * kTile) + (int)rank * kHalf, n0 = (int)(tn * BN) + (int)rank * B_ROWS;
       for (int c0 = 0; c0 < nkb && ok; c0 += a.chunk_kb) {
         const int c1 = c0 + a.chunk_kb < nkb ? c0 + a.chunk_kb : nkb;
         for (int p = 0; p < a.products && ok; ++p)
@@ -248,10 +249,10 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             ok = mbar_wait(&empty[s], phase, 21, a.dev_status, abort_flag);
             if (!ok) break;
             if (issuer) {
-              if (rank == 0) mbar_expect_tx(&full[s], 2 * (kOperandBytes + C * kBK * 2));
+              if (rank == 0) mbar_expect_tx(&full[s], 2 * (kOperandBytes + B_ROWS * kBK * 2));
               uint8_t* dst = smem + s * kStageBytes;
               load_operand<A_MN, kHalf>(dst, &tmA, m0, (kb0 + kb) * kBK, a.pa[p], full0 + s * 8);
-              load_operand<B_MN, C>(dst + kOperandBytes, &tmB, n0, (kb0 + kb) * kBK, a.pb[p], full0 + s * 8);
+              load_operand<B_MN, B_ROWS>(dst + kOperandBytes, &tmB, n0, (kb0 + kb) * kBK, a.pb[p], full0 + s * 8);
             }
             __syncwarp();
             if (++s == kStages) {
@@ -261,7 +262,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           }
       }
     }
-  } else if (warp == kDrainWarps + 1) {
+  } else if (warp == DRAIN + 1) {
     // ------------------------------------------------ MMA issuer
     if (rank == 0) {
       const bool issuer = elect_one();
@@ -306,9 +307,9 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     }
   } else {
     // ------------------------------------------------ drain + epilogue
-    const int q = warp & 3, half = warp >> 2;  // tensor-memory lane quarter; which half of the columns
+    const int q = warp & 3, part = warp >> 2;  // tensor-memory lane quarter; which columns
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
-    const Out out{smem + kOutOffset + warp * kOutBytes, lane};
+    const Out out{smem + out_offset(BN, C) + warp * kOutBytes, lane};
     uint32_t chunk = 0;
     bool ok = true;
     for (int64_t u = pair; u < units.units && ok; u += num_pairs) {
@@ -326,7 +327,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 #pragma unroll
         for (int g = 0; g < C / 16; ++g) {
           float v[16];
-          tmem_ld16_nowait(tmem_base + b * kTile + lane_base + half * C + g * 16, v);
+          tmem_ld16_nowait(tmem_base + b * kTile + lane_base + part * C + g * 16, v);
           tmem_wait_ld();
           if (g == C / 16 - 1) {
             tc_fence_before();
@@ -337,7 +338,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         }
       }
       if (!ok) break;
-      epi(acc, (int)(tm * kTile) + (int)rank * kHalf + q * 32 + lane, (int)(tn * BN) + half * C, split, &tmC, out);
+      epi(acc, (int)(tm * kTile) + (int)rank * kHalf + q * 32 + lane, (int)(tn * BN) + part * C, split, &tmC, out);
     }
     if (lane == 0) tma_store_wait_all();
   }
@@ -345,7 +346,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   tc_fence_before();
   __syncwarp();
   cluster_sync_all();  // no CTA leaves (or frees tensor memory) while its peer may still use it
-  if (warp == kDrainWarps + 1) {
+  if (warp == DRAIN + 1) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, 512);
   }
@@ -371,9 +372,11 @@ inline int tile_columns(int64_t M, int64_t N, int64_t K, int products, int sms) 
   return narrow < wide ? 128 : 256;
 }
 
+// Columns of a drain warp: 128 of a wide tile (eight warps), unless the epilogue asks for fewer (Epi::kColumns).
 template <int BN, bool A_MN, bool B_MN, class Epi>
 int launch(const Operand& A, const Operand& B, bool bf16, Args args, const CUtensorMap& tc, const Epi& epi, int device, int sms,
            cudaStream_t s) {
+  constexpr int C = Epi::kColumns < BN / 2 ? Epi::kColumns : BN / 2, BYTES = smem_bytes(BN, C);
   CUtensorMap ta, tb;
   int st = make_map(&ta, A, bf16, A_MN, kHalf);
   if (st == TCB200_OK) st = make_map(&tb, B, bf16, B_MN, BN / 2);
@@ -389,8 +392,8 @@ int launch(const Operand& A, const Operand& B, bool bf16, Args args, const CUten
   if (units == 0) return TCB200_OK;
   const unsigned pairs = (unsigned)std::min<int64_t>(units, std::max(1, sms / 2));
   static std::atomic<uint64_t> configured{0};
-  TCB200_CUDA_TRY(ensure_dynamic_smem(pair_gemm_kernel<BN, A_MN, B_MN, Epi>, kSmemBytes, device, configured));
-  TCB200_CUDA_TRY(launch_pdl(pair_gemm_kernel<BN, A_MN, B_MN, Epi>, dim3(2 * pairs), dim3(kThreads), kSmemBytes, s, ta, tb, tc, args, epi));
+  TCB200_CUDA_TRY(ensure_dynamic_smem(pair_gemm_kernel<BN, C, A_MN, B_MN, Epi>, BYTES, device, configured));
+  TCB200_CUDA_TRY(launch_pdl(pair_gemm_kernel<BN, C, A_MN, B_MN, Epi>, dim3(2 * pairs), dim3(block_threads(BN, C)), BYTES, s, ta, tb, tc, args, epi));
   return TCB200_OK;
 }
 template <bool A_MN, bool B_MN, class Epi>
