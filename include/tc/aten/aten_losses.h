@@ -73,7 +73,7 @@ inline tcb200_linear_ce_t linearCe(const at::Tensor& X, const at::Tensor& W, con
   p.ignore_index = ignoreIndex;
   p.dtype = lossType(X, "X");
   p.index_bytes = lossIndexBytes(target, "target");
-  p.pack_w = p.ldw % 8 != 0 || reinterpret_cast<uintptr_t>(W.data_ptr()) % 16 != 0;
+  p.pack_w = p.ldw * W.element_size() % 16 != 0 || reinterpret_cast<uintptr_t>(W.data_ptr()) % 16 != 0;
   return p;
 }
 

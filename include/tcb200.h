@@ -255,12 +255,12 @@ typedef struct tcb200_linear_ce {
   int64_t N, D, V;         /* X is [N, D], W is [V, D], target, loss and lse are [N] */
   int64_t ldx, ldw;        /* elements between rows of X and of W (>= D); dX and dW are dense */
   int64_t ignore_index;
-  int32_t dtype;           /* TCB200_F32 / F16 / BF16: X, W, dX, dW.  float32 is computed to fp32 accuracy (three bf16
-                              planes per operand, six products) */
+  int32_t dtype;           /* TCB200_F32 / F16 / BF16: X, W, dX, dW.  float32 is computed to fp32 accuracy */
   int32_t index_bytes;     /* 4 or 8: target is int32 or int64 */
-  int32_t pack_w;          /* f16 / bf16: 1 = rows of W may start anywhere, W is copied to aligned scratch piece by piece;
-                              0 = W is read in place, which needs W 16-byte aligned and ldw a multiple of 8, else
-                              TCB200_ERR_ALIGNMENT.  float32 always packs */
+  int32_t pack_w;          /* 0 = the rows of W start on 16-byte boundaries; 1 = anywhere.  f16 / bf16 rows are read in place
+                              with 0 (W 16-byte aligned and ldw a multiple of 8, else TCB200_ERR_ALIGNMENT) and copied to
+                              aligned scratch piece by piece with 1; float32 is split into 16-bit planes there either way,
+                              except for few rows (N <= 16), which are computed from W directly */
   int32_t reserved;        /* 0 */
 } tcb200_linear_ce_t;
 int tcb200_linear_ce_workspace(const tcb200_linear_ce_t* problem, int64_t* forward_bytes, int64_t* backward_bytes);

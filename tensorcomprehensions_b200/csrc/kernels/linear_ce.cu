@@ -71,6 +71,20 @@ int make_out_map(CUtensorMap* tm, const Operand& o, int bytes) {
   return r == CUDA_SUCCESS ? TCB200_OK : TCB200_ERR_CUDA;
 }
 
+int make_plain_map(CUtensorMap* tm, const void* base, int dtype, int64_t cols, int64_t rows, int64_t ld, int box_cols, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return TCB200_ERR_CUDA;
+  const int64_t bytes = dtype == TCB200_F32 ? 4 : 2;
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, 1};
+  cuuint64_t strides[2] = {(cuuint64_t)(ld * bytes), (cuuint64_t)(rows * ld * bytes)};
+  cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(tm, bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims,
+                  strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? TCB200_OK : TCB200_ERR_CUDA;
+}
+
 }  // namespace pg
 
 using namespace lce;
@@ -601,7 +615,7 @@ int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
   l->dw_bn = pg::tile_columns(l->bwd_piece, p.D, p.N, products, sms);
   l->few_fwd = few_forward_ok(p);
   l->few_bwd = few_backward_ok(p);
-  l->parts = l->few_fwd ? few_blocks(p, sms) : ceil_div(p.V, l->fwd_bn / 2);
+  l->parts = l->few_fwd ? few_blocks(p, sms, false) : ceil_div(p.V, l->fwd_bn / 2);
   // dX has few tiles and a long sum: the vocabulary of a piece is split where that fills the last round of the pairs.
   // Cost of S splits in k-blocks of a pair: rounds x (a unit's k-blocks + 8 for its start and epilogue) + what adding S
   // planes costs (a plane of a tile is about 4 k-blocks of memory traffic).
@@ -616,7 +630,7 @@ int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
       l->splits = (int)s;
     }
   }
-  if (l->few_bwd) l->splits = (int)few_blocks(p, sms);
+  if (l->few_bwd) l->splits = (int)few_blocks(p, sms, true);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t here = at;

@@ -58,7 +58,7 @@ struct Running {
 constexpr int kFewRows = 16;
 bool few_forward_ok(const tcb200_linear_ce_t& p);
 bool few_backward_ok(const tcb200_linear_ce_t& p);
-int64_t few_blocks(const tcb200_linear_ce_t& p, int sms);
+int64_t few_blocks(const tcb200_linear_ce_t& p, int sms, bool backward);
 int few_forward(const tcb200_linear_ce_t& p, const void* X, const void* W, const void* target, const Rows& r, float2* part,
                 float* hit, int64_t n_pad, int device, int sms, cudaStream_t s);
 int few_backward(const tcb200_linear_ce_t& p, const void* X, const void* W, const void* target, const float* lse,

@@ -8,6 +8,7 @@
 // more with a thread per column group for dW = dZ^T X and its share of dX = dZ W.  dX is summed per block in shared memory and
 // over the blocks by a second kernel, in fixed order.  dZ stays fp32, and nothing is packed.
 #include "linear_ce.cuh"
+#include "pair_gemm.cuh"
 
 namespace tcb200 {
 namespace lce {
@@ -15,7 +16,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kForwardSmem = 100 << 10;        // two blocks an SM at least
+constexpr int kForwardSmem = 92 << 10;         // X: two blocks an SM at least, or one and the ring
 constexpr int kBackwardSmem = 200 << 10;       // X and dX
 
 // vocabulary entries a warp takes at a time: its sums are at most 32, one a lane in the end
@@ -88,6 +89,29 @@ __device__ __forceinline__ void stage_x(const Few& f, const T* x, float* sx) {
   }
 }
 
+// The list acc, one per lane, summed over the warp: lane l gets value l / (32 / N).  Halves of the list change sides until a
+// lane holds one value, then the rest of the lanes are added.
+template <int N>
+__device__ __forceinline__ float spread(float (&acc)[N], int lane) {
+  int n = N;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    if (n > 1) {
+      n /= 2;
+      const bool up = lane & o;
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i)
+        if (i < n) {
+          const float keep = up ? acc[i + n] : acc[i], send = up ? acc[i] : acc[i + n];
+          acc[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+    } else {
+      acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], o);
+    }
+  }
+  return acc[0];
+}
+
 // A warp's entries of W as a stream of chunks, always one chunk ahead: the loads of a chunk are under way while the one before
 // is multiplied, from one group of entries to the next too.
 template <typename T, bool VEC, int PER>
@@ -131,24 +155,7 @@ __device__ __forceinline__ float logits_of(Stream<T, VEC, entries(NR)>& st, int6
         for (int j = 0; j < E; ++j) acc[r * PER + e] = fmaf(xv[j], wv[e][j], acc[r * PER + e]);
     }
   }
-  // halves of the list change sides until a lane holds one value, then the rest of the lanes are added
-  int n = NR * PER;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    if (n > 1) {
-      n /= 2;
-      const bool up = st.lane & o;
-#pragma unroll
-      for (int i = 0; i < NR * PER / 2; ++i)
-        if (i < n) {
-          const float keep = up ? acc[i + n] : acc[i], send = up ? acc[i] : acc[i + n];
-          acc[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-        }
-    } else {
-      acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], o);
-    }
-  }
-  return acc[0];
+  return spread<NR * PER>(acc, st.lane);
 }
 
 // blocks of an SM: registers for the chunk ahead and the sums
@@ -191,6 +198,120 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NR)) few_forward_kerne
     for (int k = 0; k < kWarps; ++k)
       for (int i = 0; i < PER; ++i) all.join(pairs[k][(threadIdx.x * PER + i) * SHARE]);
     part[blockIdx.x * n_pad + threadIdx.x] = make_float2(all.top, all.sum);
+  }
+}
+
+// Forward where the rows of W start on 16-byte boundaries: a producer warp keeps a ring of boxes (32 entries x 512 bytes) full
+// with TMA loads, 128 KB of them under way, and eight warps multiply, four entries each.  The plain loads above keep a
+// quarter of that in flight (1 x 4096 x 128000 bf16: 560 us; this kernel 162 us, 6.5 TB/s).
+constexpr int kRing = 8, kBoxRows = 32, kBoxBytes = kBoxRows * 512;
+__host__ __device__ constexpr int ring_bytes() { return kRing * kBoxBytes + 128; }
+constexpr int kRingSmem = ring_bytes() + kForwardSmem;
+static_assert(kRingSmem <= 224 * 1024, "the ring and X exceed shared memory");
+template <int NR, typename T>
+__global__ void __launch_bounds__(kThreads + 32, 1) few_ring_kernel(const __grid_constant__ CUtensorMap tm, Few f, const T* x, Rows rows,
+                                                                    float2* part, float* hit, int64_t n_pad) {
+  constexpr int E = Step<T>::E, CHUNK = Step<T>::CHUNK, PER = 4, SHARE = 32 / (NR * PER);
+  static_assert(CHUNK * sizeof(T) == 512 && kWarps * PER == kBoxRows, "a box is a chunk of the block's entries");
+  extern __shared__ __align__(128) uint8_t ring[];
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kRing * kBoxBytes);
+  uint64_t* empty = full + kRing;
+  float* sx = reinterpret_cast<float*>(ring + ring_bytes());
+  __shared__ float2 pairs[kWarps][32];
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dp = (int)padded(f.d);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kRing; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], kWarps);
+    }
+    abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  pdl_sync();
+  if (blockIdx.x == 0 && threadIdx.x < f.n) {
+    const int64_t t = f.index(threadIdx.x);
+    rows.place[threadIdx.x] = t != f.ignore ? (int)threadIdx.x : -1;
+    rows.target[threadIdx.x] = t >= 0 && t < f.v ? (int)t : -1;
+    if (threadIdx.x == 0) *rows.head = Head{(int)f.n, 0, 1.f};
+  }
+  int* status = &rows.head->status;
+  const int groups = (int)((f.v + kBoxRows - 1) / kBoxRows), chunks = (int)((f.d + CHUNK - 1) / CHUNK);
+  if (warp == kWarps) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t phase = 1;
+      bool ok = true;
+      for (int g = blockIdx.x; g < groups && ok; g += gridDim.x)
+        for (int c = 0; c < chunks; ++c) {
+          ok = mbar_wait(&empty[s], phase, 31, status, abort_flag);
+          if (!ok) break;
+          mbar_expect_tx(&full[s], kBoxBytes);
+          tma_load_3d(ring + s * kBoxBytes, &tm, c * CHUNK, g * kBoxRows, 0, &full[s]);
+          if (++s == kRing) {
+            s = 0;
+            phase ^= 1;
+          }
+        }
+    }
+  } else {
+    stage_x<NR>(f, x, sx);
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");  // the multiplying warps
+    const int value = lane / SHARE, r = value / PER, e = value % PER;
+    const int64_t t = r < f.n ? f.index(r) : -1;
+    Running run;
+    int s = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int g = blockIdx.x; g < groups && ok; g += gridDim.x) {
+      float acc[NR * PER];
+#pragma unroll
+      for (int i = 0; i < NR * PER; ++i) acc[i] = 0.f;
+      for (int c = 0; c < chunks; ++c) {
+        ok = mbar_wait(&full[s], phase, 32, status, abort_flag);
+        if (!ok) break;
+        const T* box = reinterpret_cast<const T*>(ring + s * kBoxBytes) + warp * PER * CHUNK + lane * E;
+        Raw<T> now[PER];
+#pragma unroll
+        for (int k = 0; k < PER; ++k) *reinterpret_cast<uint4*>(&now[k]) = *reinterpret_cast<const uint4*>(box + k * CHUNK);
+        float wv[PER][E];
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+#pragma unroll
+          for (int j = 0; j < E; ++j) wv[k][j] = to_float(now[k].v[j]);
+        mbar_arrive_warp(&empty[s]);  // the box is in registers
+        if (++s == kRing) {
+          s = 0;
+          phase ^= 1;
+        }
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+          float xv[E];
+          load_x<T, true>(sx + i * dp, c * CHUNK, lane, xv);
+#pragma unroll
+          for (int k = 0; k < PER; ++k)
+#pragma unroll
+            for (int j = 0; j < E; ++j) acc[i * PER + k] = fmaf(xv[j], wv[k][j], acc[i * PER + k]);
+        }
+      }
+      if (!ok) break;
+      const float z = spread<NR * PER>(acc, lane);
+      const int64_t v = (int64_t)g * kBoxRows + warp * PER + e;
+      if (lane % SHARE == 0 && r < f.n && v < f.v) {
+        run.join(make_float2(z, 1.f));
+        if (v == t) hit[r] = z;
+      }
+    }
+    pairs[warp][lane] = make_float2(run.top, run.sum);
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+    if (threadIdx.x < f.n) {
+      Running all;
+      for (int k = 0; k < kWarps; ++k)
+        for (int i = 0; i < PER; ++i) all.join(pairs[k][(threadIdx.x * PER + i) * SHARE]);
+      part[blockIdx.x * n_pad + threadIdx.x] = make_float2(all.top, all.sum);
+    }
   }
 }
 
@@ -319,12 +440,28 @@ Few few_of(const tcb200_linear_ce_t& p, const void* target) {
   return {target, p.index_bytes, p.ignore_index, p.N, p.D, p.V, p.ldx, p.ldw};
 }
 
+bool aligned_rows(const void* base, int64_t ld, size_t bytes) { return ((uintptr_t)base & 15) == 0 && ld * bytes % 16 == 0; }
+
+template <int NR, typename T>
+int ring_launch(const tcb200_linear_ce_t& p, const void* X, const void* W, const void* target, const Rows& r, float2* part,
+                float* hit, int64_t n_pad, int device, int sms, cudaStream_t s) {
+  CUtensorMap tm;
+  const int st = pg::make_plain_map(&tm, W, p.dtype, p.D, p.V, p.ldw, Step<T>::CHUNK, kBoxRows);
+  if (st != TCB200_OK) return st;
+  static std::atomic<uint64_t> configured{0};
+  TCB200_CUDA_TRY(ensure_dynamic_smem(few_ring_kernel<NR, T>, kRingSmem, device, configured));
+  TCB200_CUDA_TRY(launch_pdl(few_ring_kernel<NR, T>, dim3((unsigned)few_blocks(p, sms, false)), dim3(kThreads + 32),
+                             (size_t)(ring_bytes() + forward_smem(p)), s, tm, few_of(p, target), static_cast<const T*>(X), r, part, hit,
+                             n_pad));
+  return TCB200_OK;
+}
+
 template <int NR, bool VEC, typename T>
 int forward_launch(const tcb200_linear_ce_t& p, const void* X, const void* W, const void* target, const Rows& r, float2* part,
                    float* hit, int64_t n_pad, int device, int sms, cudaStream_t s) {
   static std::atomic<uint64_t> configured{0};
   TCB200_CUDA_TRY(ensure_dynamic_smem(few_forward_kernel<NR, VEC, T>, kForwardSmem, device, configured));
-  TCB200_CUDA_TRY(launch_pdl(few_forward_kernel<NR, VEC, T>, dim3((unsigned)few_blocks(p, sms)), dim3(kThreads),
+  TCB200_CUDA_TRY(launch_pdl(few_forward_kernel<NR, VEC, T>, dim3((unsigned)few_blocks(p, sms, false)), dim3(kThreads),
                              (size_t)forward_smem(p), s, few_of(p, target), static_cast<const T*>(X), static_cast<const T*>(W), r,
                              part, hit, n_pad));
   return TCB200_OK;
@@ -335,42 +472,62 @@ int backward_launch(const tcb200_linear_ce_t& p, const void* X, const void* W, c
                     void* dW, int device, int sms, cudaStream_t s) {
   static std::atomic<uint64_t> configured{0};
   TCB200_CUDA_TRY(ensure_dynamic_smem(few_backward_kernel<NR, VEC, T>, kBackwardSmem, device, configured));
-  TCB200_CUDA_TRY(launch_pdl(few_backward_kernel<NR, VEC, T>, dim3((unsigned)few_blocks(p, sms)), dim3(kThreads),
+  TCB200_CUDA_TRY(launch_pdl(few_backward_kernel<NR, VEC, T>, dim3((unsigned)few_blocks(p, sms, true)), dim3(kThreads),
                              (size_t)(2 * forward_smem(p)), s, few_of(p, target), static_cast<const T*>(X),
                              static_cast<const T*>(W), lse, g, g_stride, r, sums, plane, ld, static_cast<T*>(dW), (int)(dX != nullptr)));
   if (dX)
     TCB200_CUDA_TRY(launch_pdl(few_finish_kernel<T>, dim3((unsigned)ceil_div(p.D, 32), (unsigned)p.N), dim3(32, 32), 0, s, r,
-                               static_cast<const float*>(sums), (int)few_blocks(p, sms), plane, ld, p.D, static_cast<T*>(dX)));
+                               static_cast<const float*>(sums), (int)few_blocks(p, sms, true), plane, ld, p.D, static_cast<T*>(dX)));
   return TCB200_OK;
 }
 
-bool aligned_rows(const void* base, int64_t ld, size_t bytes) { return ((uintptr_t)base & 15) == 0 && ld * bytes % 16 == 0; }
-
-// 16-bit types come here with rows that start anywhere
-#define TCB200_FEW_CASE(NR, CALL)                                                                     \
-  case NR:                                                                                             \
-    if (p.dtype == TCB200_F32) return vec ? CALL<NR, true, float> ARGS : CALL<NR, false, float> ARGS; \
-    if (p.dtype == TCB200_F16) return CALL<NR, false, __half> ARGS;                                   \
+// 16-bit types come here with rows that start anywhere; float32 rows of that kind too, or (F32VEC) any
+#define TCB200_FEW_CASE(NR, CALL, F32VEC)                                                                       \
+  case NR:                                                                                                       \
+    if (p.dtype == TCB200_F32) return F32VEC && vec ? CALL<NR, F32VEC, float> ARGS : CALL<NR, false, float> ARGS; \
+    if (p.dtype == TCB200_F16) return CALL<NR, false, __half> ARGS;                                             \
     return CALL<NR, false, __nv_bfloat16> ARGS;
 
 }  // namespace
 
 // 4 x 2048 x 50000 float32, forward and gradient: 355 us here, 1155 us on the tensor cores; 6 x 92 x 38224 f16 with rows to be
 // packed 91 and 136 us; 8 x 2048 x 50000 bf16 with aligned rows 546 and 224 us.
+// The ring needs rows on 16-byte boundaries.  16-bit rows of W need no packing for the tensor cores either, which win from five
+// rows up (8 x 2048 x 50000 bf16, forward: 56 us, here 83 us; one row of 4096 x 128000: 203 and 162 us).
+bool ring_ok(const tcb200_linear_ce_t& p) {
+  return p.N <= (p.dtype == TCB200_F32 ? 8 : 4) && !p.pack_w && p.ldw * (p.dtype == TCB200_F32 ? 4 : 2) % 16 == 0;
+}
 bool few_rows(const tcb200_linear_ce_t& p) { return p.dtype == TCB200_F32 ? p.N <= kFewRows : p.pack_w && p.N <= kFewRows / 2; }
-bool few_forward_ok(const tcb200_linear_ce_t& p) { return few_rows(p) && forward_smem(p) <= kForwardSmem; }
+bool few_forward_ok(const tcb200_linear_ce_t& p) { return (few_rows(p) || ring_ok(p)) && forward_smem(p) <= kForwardSmem; }
 bool few_backward_ok(const tcb200_linear_ce_t& p) { return few_rows(p) && 2 * forward_smem(p) <= kBackwardSmem; }
-int64_t few_blocks(const tcb200_linear_ce_t& p, int sms) { return std::min<int64_t>(ceil_div(p.V, kWarps * entries(padded_rows(p.N))), (int64_t)sms * blocks_per_sm((int)padded_rows(p.N))); }
+int64_t few_blocks(const tcb200_linear_ce_t& p, int sms, bool backward) {
+  const int nr = padded_rows(p.N);
+  const int64_t per_sm = backward ? 2 : ring_ok(p) ? 1 : blocks_per_sm(nr);
+  return std::min<int64_t>(ceil_div(p.V, kWarps * entries(nr)), sms * per_sm);
+}
 
 int few_forward(const tcb200_linear_ce_t& p, const void* X, const void* W, const void* target, const Rows& r, float2* part,
                 float* hit, int64_t n_pad, int device, int sms, cudaStream_t s) {
   const bool vec = aligned_rows(W, p.ldw, p.dtype == TCB200_F32 ? 4 : 2);
 #define ARGS (p, X, W, target, r, part, hit, n_pad, device, sms, s)
+  if (vec && ring_ok(p)) {
+#define TCB200_RING_CASE(NR)                                      \
+  case NR:                                                        \
+    if (p.dtype == TCB200_F32) return ring_launch<NR, float> ARGS; \
+    if (p.dtype == TCB200_F16) return ring_launch<NR, __half> ARGS; \
+    return ring_launch<NR, __nv_bfloat16> ARGS;
+    switch (padded_rows(p.N)) {
+      TCB200_RING_CASE(1)
+      TCB200_RING_CASE(2)
+      TCB200_RING_CASE(4)
+      TCB200_RING_CASE(8)
+    }
+  }
   switch (padded_rows(p.N)) {
-    TCB200_FEW_CASE(1, forward_launch)
-    TCB200_FEW_CASE(2, forward_launch)
-    TCB200_FEW_CASE(4, forward_launch)
-    TCB200_FEW_CASE(8, forward_launch)
+    TCB200_FEW_CASE(1, forward_launch, false)
+    TCB200_FEW_CASE(2, forward_launch, false)
+    TCB200_FEW_CASE(4, forward_launch, false)
+    TCB200_FEW_CASE(8, forward_launch, false)
     case 16: return vec ? forward_launch<16, true, float> ARGS : forward_launch<16, false, float> ARGS;
   }
 #undef ARGS
@@ -385,10 +542,10 @@ int few_backward(const tcb200_linear_ce_t& p, const void* X, const void* W, cons
   const bool vec = aligned_rows(W, p.ldw, bytes) && aligned_rows(dW, p.D, bytes);
 #define ARGS (p, X, W, target, lse, g, g_stride, r, sums, plane, ld, dX, dW, device, sms, s)
   switch (padded_rows(p.N)) {
-    TCB200_FEW_CASE(1, backward_launch)
-    TCB200_FEW_CASE(2, backward_launch)
-    TCB200_FEW_CASE(4, backward_launch)
-    TCB200_FEW_CASE(8, backward_launch)
+    TCB200_FEW_CASE(1, backward_launch, true)
+    TCB200_FEW_CASE(2, backward_launch, true)
+    TCB200_FEW_CASE(4, backward_launch, true)
+    TCB200_FEW_CASE(8, backward_launch, true)
     case 16: return vec ? backward_launch<16, true, float> ARGS : backward_launch<16, false, float> ARGS;
   }
 #undef ARGS

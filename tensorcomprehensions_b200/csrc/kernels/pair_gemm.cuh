@@ -361,6 +361,8 @@ struct Operand {
 int make_map(CUtensorMap* tm, const Operand& o, bool bf16, bool mn_major, int rows);
 // An output [planes][rows][cols] of 2- or 4-byte elements, written in boxes of 32 rows x 128 bytes.
 int make_out_map(CUtensorMap* tm, const Operand& o, int bytes);
+// A matrix of `dtype` elements read in boxes without a swizzle (zeros out of bounds); base and row stride multiples of 16 bytes.
+int make_plain_map(CUtensorMap* tm, const void* base, int dtype, int64_t cols, int64_t rows, int64_t ld, int box_cols, int box_rows);
 
 // Columns of a tile: 128 where that finishes earlier, which is where tiles of 256 leave pairs without work.  A k-block takes a
 // pair about 530 cycles with 256 columns and 400 with 128 (the loads, not the MMAs, bound it then); a unit's start, drain

@@ -183,21 +183,27 @@ struct Running {
   }
 };
 
-// All threads get the block's pairs (two at once, of two scales); `share` holds two pairs a warp.  Pairs are joined in a
-// fixed order.
-__device__ __forceinline__ void block_join(Running& a, float scale_a, Running& b, float scale_b, float4* share) {
-  for (int o = 16; o; o >>= 1) {
-    a.join(__shfl_xor_sync(0xffffffffu, a.top, o), __shfl_xor_sync(0xffffffffu, a.sum, o), scale_a);
-    b.join(__shfl_xor_sync(0xffffffffu, b.top, o), __shfl_xor_sync(0xffffffffu, b.sum, o), scale_b);
-  }
+// The pair of a whole warp: the maximum first, then the sums moved to it, so that the shuffles carry one exponential.
+__device__ __forceinline__ Running warp_join(Running r, float scale) {
+  float m = r.top;
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  r.raise(m, scale);
+  for (int o = 16; o; o >>= 1) r.sum += __shfl_xor_sync(0xffffffffu, r.sum, o);
+  return r;
+}
+// All threads get the block's pairs (two at once); `share` holds two pairs a warp.  Pairs are joined in a fixed order.
+__device__ __forceinline__ void block_join(Running& a, Running& b, float scale, float4* share) {
+  a = warp_join(a, scale);
+  b = warp_join(b, scale);
   if ((threadIdx.x & 31) == 0) share[threadIdx.x >> 5] = make_float4(a.top, a.sum, b.top, b.sum);
   __syncthreads();
-  a = b = Running();
-  for (int w = 0; w < kThreads / 32; ++w) {
-    const float4 x = share[w];
-    a.join(x.x, x.y, scale_a);
-    b.join(x.z, x.w, scale_b);
-  }
+  // every warp joins the warps' pairs, a lane each
+  const int lane = threadIdx.x & 31;
+  const float4 x = lane < kThreads / 32 ? share[lane] : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+  a.top = x.x; a.sum = x.y;
+  b.top = x.z; b.sum = x.w;
+  a = warp_join(a, scale);
+  b = warp_join(b, scale);
 }
 
 // [first, last) of a row for part `i` of `n`: whole 64-element steps, so that the parts' inner bounds keep the alignment of the row
@@ -258,7 +264,7 @@ __global__ void __launch_bounds__(kThreads) distill_forward_kernel(const T* logi
       bad |= at >= v;
       if (at >= 0) t.one<float>(e.logit(row, j), scale);
     }
-  block_join(r, scale, t, scale, share);
+  block_join(r, t, scale, share);
   if (parts > 1) {
     if (threadIdx.x == 0) {
       uint32_t at;
