@@ -81,3 +81,20 @@ def test_tensors_off_the_device_are_refused():
         tc.linear_cross_entropy(x, w, t)
     with pytest.raises(RuntimeError, match="logits must be a CUDA tensor"):
         tc.topk_distillation(torch.zeros(4, 16), torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, 2))
+
+
+def test_cpp_entry_points_without_a_device():
+    if torch.cuda.is_available():
+        pytest.skip("covered by the gpu variant")
+    from test_cpp_api import _build, _run
+    r = _run(_build("losses"))
+    assert r.returncode == 0, r.stdout + r.stderr
+    assert "losses ok (gpu=0)" in r.stdout
+
+
+@pytest.mark.gpu
+def test_cpp_entry_points(cuda):
+    from test_cpp_api import _build, _run
+    r = _run(_build("losses"))
+    assert r.returncode == 0, r.stdout + r.stderr
+    assert "losses ok (gpu=1)" in r.stdout

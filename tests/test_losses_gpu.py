@@ -220,6 +220,97 @@ def test_empty_batch(cuda):
         assert loss.shape == (0,) and dx.shape == (0, 32) and (dw == 0).all()
 
 
+def test_strided_gradient_and_saved_inputs(cuda):
+    x, w, t, up = make_ce(cuda, 50, 40, 90, torch.float32)
+    want = step_ce(x, w, t, up)
+    wide = torch.full((50, 3), float("nan"), device=cuda)
+    wide[:, 1] = up
+    for a, b in zip(want, step_ce(x, w, t, wide[:, 1])):
+        assert torch.equal(a, b)
+    x.requires_grad_()
+    loss = tc.linear_cross_entropy(x, w, t)
+    w.mul_(2)  # the backward pass would read another W than the forward did
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.sum().backward()
+    # no second derivative
+    (dx,) = torch.autograd.grad(tc.linear_cross_entropy(x, w, t).sum(), x, retain_graph=True)
+    assert not dx.requires_grad
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(tc.linear_cross_entropy(x, w, t).sum(), x, create_graph=True)
+    z, i, s, _ = make_kd(cuda, 4, 50, 3, torch.float32)
+    z.requires_grad_()
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(tc.topk_distillation(z, i, s).sum(), z, create_graph=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,d,v", [(1, 64, 100), (3, 33, 65), (20, 72, 300), (300, 45, 513), (257, 264, 1000)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_nothing_is_written_outside_the_outputs(cuda, dtype, n, d, v, shift):
+    """The C entry points with every buffer between two guards, dX and dW on and off their 16-byte boundaries."""
+    import ctypes
+    from tensorcomprehensions_b200 import cabi
+    x, w, t, up = make_ce(cuda, n, d, v, dtype, 0.2)
+    size = x.element_size()
+    code = {torch.float32: cabi.F32, torch.float16: cabi.F16, torch.bfloat16: cabi.BF16}[dtype]
+    p = cabi.LinearCe(n, d, v, d, d, -100, code, 8, int(d * size % 16 != 0), 0)
+    f, b = ctypes.c_int64(), ctypes.c_int64()
+    cabi.check(cabi.lib().tcb200_linear_ce_workspace(ctypes.byref(p), ctypes.byref(f), ctypes.byref(b)), "workspace")
+    GUARD = 4096
+
+    def guarded(nbytes, offset=0):
+        buf = torch.full((GUARD + offset + nbytes + GUARD,), 0xCD, device=cuda, dtype=torch.uint8)
+        return buf, GUARD + offset, nbytes
+
+    def untouched(g):
+        buf, at, nbytes = g
+        return bool((buf[:at] == 0xCD).all()) and bool((buf[at + nbytes:] == 0xCD).all())
+
+    def ptr(g):
+        return ctypes.c_void_p(g[0].data_ptr() + g[1])
+
+    def values(g, dt, shape):
+        return g[0][g[1]:g[1] + g[2]].clone().view(dt).view(shape)
+
+    loss, lse, wf, wb = guarded(4 * n), guarded(4 * n), guarded(f.value), guarded(b.value)
+    dx, dw = guarded(n * d * size, shift * size), guarded(v * d * size, shift * size)
+    st = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    P = lambda a: ctypes.c_void_p(a.data_ptr())  # noqa: E731
+    cabi.check(cabi.lib().tcb200_linear_ce_forward(ctypes.byref(p), P(x), P(w), P(t), ptr(loss), ptr(lse), ptr(wf), f.value, st, None), "forward")
+    cabi.check(cabi.lib().tcb200_linear_ce_backward(ctypes.byref(p), P(x), P(w), P(t), ptr(lse), P(up), 1, ptr(dx), ptr(dw), ptr(wb), b.value, st, None), "backward")
+    torch.cuda.synchronize()
+    assert all(untouched(g) for g in (loss, lse, wf, wb, dx, dw))
+    check_ce(x, w, t, up, values(loss, torch.float32, (n,)), values(dx, dtype, (n, d)), values(dw, dtype, (v, d)))
+
+
+@pytest.mark.parametrize("n", [3, 40])
+def test_offsets_behind_32_bits(cuda, n):
+    """W and dW of 2.4e9 elements: single entries behind the 2^31st against 64 bits."""
+    d, v = 4096, 590000
+    g = torch.Generator(device=cuda).manual_seed(3)
+    x = torch.randn(n, d, generator=g, device=cuda).bfloat16()
+    w = torch.empty(v, d, device=cuda, dtype=torch.bfloat16).normal_(0, 1 / 64, generator=g)
+    t = torch.randint(v - 1000, v, (n,), generator=g, device=cuda)
+    up = torch.rand(n, generator=g, device=cuda)
+    loss, dx, dw = step_ce(x, w, t, up)
+    X = x.double()
+    z = torch.cat([X @ w[a:a + 50000].double().t() for a in range(0, v, 50000)], 1)
+    lse = torch.logsumexp(z, 1)
+    rl = lse - z[torch.arange(n, device=cuda), t]
+    assert ((loss.double() - rl).abs() <= 2.0**-14 * (1 + rl)).all()
+    dz = torch.exp(z - lse[:, None])
+    dz[torch.arange(n, device=cuda), t] -= 1
+    dz *= up.double()[:, None]
+    rows = torch.cat([t, torch.tensor([0, v // 2, v - 1], device=cuda)])
+    rw = dz[:, rows].t() @ X
+    # dZ and dW are rounded to bfloat16, half a step 2^-8 each; the probabilities are off by 2^-10
+    tol = dz[:, rows].abs().t() @ X.abs() * (2.0**-8 + 2.0**-10) + 2.0**-8 * rw.abs()
+    assert ((dw[rows].double() - rw).abs() <= tol).all()
+    rx = sum(dz[:, a:a + 50000] @ w[a:a + 50000].double() for a in range(0, v, 50000))
+    tol = sum(dz[:, a:a + 50000].abs() @ w[a:a + 50000].double().abs() for a in range(0, v, 50000)) * (2.0**-8 + 2.0**-10) + 2.0**-8 * rx.abs()
+    assert ((dx.double() - rx).abs() <= tol).all()
+
+
 # ---------------------------------------------------------------------------------- distillation
 def make_kd(cuda, n, v, k, dtype, ragged=False, index=torch.int64, seed=0, teacher_dtype=None):
     g = torch.Generator(device=cuda).manual_seed(seed)
@@ -360,6 +451,38 @@ def test_distillation_empty_batch(cuda):
     z = torch.empty(0, 100, device=cuda)
     loss, dz = step_kd(z, torch.empty(0, 3, device=cuda, dtype=torch.int64), torch.empty(0, 3, device=cuda), torch.empty(0, device=cuda))
     assert loss.shape == (0,) and dz.shape == (0, 100)
+
+
+def test_distillation_offsets_behind_32_bits(cuda):
+    n, v, k = 17000, 131072, 5
+    g = torch.Generator(device=cuda).manual_seed(4)
+    z = torch.empty(n, v, device=cuda, dtype=torch.bfloat16).normal_(0, 2, generator=g)
+    i = torch.randint(0, v, (n, k), generator=g, device=cuda)
+    s = torch.randn(n, k, generator=g, device=cuda)
+    up = torch.rand(n, generator=g, device=cuda)
+    loss, dz = step_kd(z, i, s, up)
+    rows = torch.tensor([0, 8191, 16383, 16384, 16999], device=cuda)
+    check_kd(z[rows], i[rows], s[rows], up[rows], 1.0, loss[rows], dz[rows])
+
+
+def test_distillation_writes_nothing_outside_its_output(cuda):
+    import ctypes
+    from tensorcomprehensions_b200 import cabi
+    for dtype, code in ((torch.float32, cabi.F32), (torch.bfloat16, cabi.BF16)):
+        for n, v, k, shift in ((3, 5001, 7, 0), (3, 5001, 7, 1), (1, 40000, 300, 0), (9, 17, 4, 1)):
+            z, i, s, up = make_kd(cuda, n, v, k, dtype, True)
+            p = cabi.TopkDistill(n, v, k, v, k, k, 2.0, code, code, 8)
+            size, P = z.element_size(), (lambda a: ctypes.c_void_p(a.data_ptr()))
+            st = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+            bufs = [torch.full((4096 + o + b + 4096,), 0xCD, device=cuda, dtype=torch.uint8) for o, b in ((0, 4 * n), (0, 12 * n), (shift * size, n * v * size))]
+            loss, stats, dz = (ctypes.c_void_p(b.data_ptr() + 4096 + o) for b, o in zip(bufs, (0, 0, shift * size)))
+            cabi.check(cabi.lib().tcb200_topk_distill_forward(ctypes.byref(p), P(z), P(i), P(s), loss, stats, st), "forward")
+            cabi.check(cabi.lib().tcb200_topk_distill_backward(ctypes.byref(p), P(z), P(i), P(s), stats, P(up), 1, dz, st), "backward")
+            torch.cuda.synchronize()
+            for b, o, nb in zip(bufs, (0, 0, shift * size), (4 * n, 12 * n, n * v * size)):
+                assert (b[:4096 + o] == 0xCD).all() and (b[4096 + o + nb:] == 0xCD).all()
+            got = [b[4096 + o:4096 + o + nb].clone() for b, o, nb in zip(bufs, (0, 0, shift * size), (4 * n, 12 * n, n * v * size))]
+            check_kd(z, i, s, up, 2.0, got[0].view(torch.float32), got[2].view(dtype).view(n, v))
 
 
 # ---------------------------------------------------------------------------------- together, as they are used
