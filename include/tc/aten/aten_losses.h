@@ -34,6 +34,7 @@ inline int32_t lossType(const at::Tensor& t, const char* what) {
 inline void lossMatrix(const at::Tensor& t, const char* what, const at::Tensor& like) {
   TC_CHECK(t.is_cuda()) << what << " must be a CUDA tensor";
   TC_CHECK(t.get_device() == like.get_device()) << what << " is on another device";
+  TC_CHECK(!t.is_neg()) << what << " is a negated view: call resolve_neg() first";
   TC_CHECK_EQ(t.dim(), 2) << what << " must have two dimensions";
   TC_CHECK(t.size(1) <= 1 || t.stride(1) == 1) << what << " must be dense along its last dimension";
   TC_CHECK(t.size(0) <= 1 || t.stride(0) >= t.size(1)) << what << " has overlapping rows";

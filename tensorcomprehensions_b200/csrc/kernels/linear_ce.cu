@@ -325,7 +325,7 @@ __device__ __forceinline__ void unscale(float (&acc)[C], const float* row_factor
   const float f = row_factor[row];
 #pragma unroll
   for (int j = 0; j < C; j += 4) {
-    const float4 q = __ldg(reinterpret_cast<const float4*>(col_factor + col0 + j));
+    const float4 q = *reinterpret_cast<const float4*>(col_factor + col0 + j);
     acc[j] *= f * q.x; acc[j + 1] *= f * q.y; acc[j + 2] *= f * q.z; acc[j + 3] *= f * q.w;
   }
 }
@@ -623,7 +623,8 @@ int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
   const int64_t kb = ceil_div(l->bwd_piece, pg::kBK) * products;
   int64_t best = INT64_MAX;
   l->splits = 1;
-  for (int64_t s = 1; s <= 64 && s * 8 <= kb; ++s) {
+  // planes of at most 256 MiB
+  for (int64_t s = 1; s == 1 || (s <= 64 && s * 8 <= kb && s * l->n_pad * l->dp * 4 <= kPieceBytes); ++s) {
     const int64_t cost = ceil_div(tiles * s, pairs) * (ceil_div(kb, s) + 8) + s * (9 * tiles / pairs + 1);
     if (cost < best) {
       best = cost;

@@ -50,13 +50,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// Eight 16-bit or four 32-bit elements of 16 bytes.  scaled(x): (x - top) * scale.  float32 subtracts first, which is exact
-// where exp is not small; in 16 bits the product is folded into one multiply-add, whose error (2^-24 of |top| * scale) is far
-// below the elements' own.
+// Eight 16-bit or four 32-bit elements of 16 bytes.
 template <typename T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int n = 4;
-  static constexpr bool exact = true;
   static __device__ __forceinline__ float maximum(const uint4& r) {
     return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
   }
@@ -69,7 +66,6 @@ template <> struct Vec<float> {
 };
 template <> struct Vec<__half> {
   static constexpr int n = 8;
-  static constexpr bool exact = false;
   static __device__ __forceinline__ float maximum(const uint4& r) {
     const __half2* h = reinterpret_cast<const __half2*>(&r);
     const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
@@ -95,7 +91,6 @@ template <> struct Vec<__half> {
 };
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int n = 8;
-  static constexpr bool exact = false;
   static __device__ __forceinline__ float maximum(const uint4& r) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
     const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
@@ -138,10 +133,9 @@ struct Entries {
   }
 };
 
-template <typename T>
-__device__ __forceinline__ float exp_from(float x, float top, float neg_top_scaled, float scale) {
-  return exp2_fast(Vec<T>::exact ? (x - top) * scale : fmaf(x, scale, neg_top_scaled));
-}
+// exp((x - top) * T^-1).  The difference is taken first: it is exact where exp is not small, and rows of a type's lowest value
+// neither overflow nor lose their sum, as x * scale - top * scale in one multiply-add would.
+__device__ __forceinline__ float exp_from(float x, float top, float scale) { return exp2_fast((x - top) * scale); }
 
 // Running maximum and sum of exp((x - maximum) * scale).  An empty pair is (-inf, 0).  A maximum drops NaN; the sum keeps it.
 struct Running {
@@ -158,11 +152,9 @@ struct Running {
       top = m;
     }
   }
-  template <typename T>
   __device__ __forceinline__ void one(float x, float scale) {
     raise(x, scale);
-    const float shift = top == -INFINITY ? 0.f : top;
-    sum += exp_from<T>(x, shift, -shift * scale, scale);
+    sum += exp_from(x, top == -INFINITY ? 0.f : top, scale);
   }
   template <typename T, int U>
   __device__ __forceinline__ void vectors(const uint4 (&raw)[U], float scale) {
@@ -170,14 +162,14 @@ struct Running {
 #pragma unroll
     for (int u = 1; u < U; ++u) m = fmaxf(m, Vec<T>::maximum(raw[u]));
     raise(m, scale);
-    const float shift = top == -INFINITY ? 0.f : top, neg = -shift * scale;
+    const float shift = top == -INFINITY ? 0.f : top;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float x[Vec<T>::n];
       Vec<T>::unpack(raw[u], x);
 #pragma unroll
-      for (int j = 0; j < Vec<T>::n; ++j) s[j & 3] += exp_from<T>(x[j], shift, neg, scale);
+      for (int j = 0; j < Vec<T>::n; ++j) s[j & 3] += exp_from(x[j], shift, scale);
     }
     sum += (s[0] + s[1]) + (s[2] + s[3]);
   }
@@ -250,19 +242,19 @@ __global__ void __launch_bounds__(kThreads) distill_forward_kernel(const T* logi
     const uint4 raw[1] = {load_raw(body + (int64_t)i * W)};
     r.vectors<T, 1>(raw, scale);
   }
-  if (first + threadIdx.x < head) r.one<T>(load1(z + first + threadIdx.x), scale);
+  if (first + threadIdx.x < head) r.one(load1(z + first + threadIdx.x), scale);
   const int64_t rest = head + (int64_t)vecs * W + threadIdx.x;
-  if (rest < last) r.one<T>(load1(z + rest), scale);
+  if (rest < last) r.one(load1(z + rest), scale);
   // the entries' maximum and sum go along with the row's
   const float student = place >= 0 && place < v ? load1(z + place) : 0.f;
   bool bad = place >= v;
   Running t;
-  if (place >= 0) t.one<float>(teacher, scale);
+  if (place >= 0) t.one(teacher, scale);
   if (rank == 0)
     for (int j = threadIdx.x + kThreads; j < e.k; j += kThreads) {
       const int64_t at = e.index(row, j);
       bad |= at >= v;
-      if (at >= 0) t.one<float>(e.logit(row, j), scale);
+      if (at >= 0) t.one(e.logit(row, j), scale);
     }
   block_join(r, t, scale, share);
   if (parts > 1) {
@@ -329,8 +321,7 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const T* log
   }
   constexpr int W = Vec<T>::n;
   const float weight = up / sum;
-  const float neg = -top * scale;
-  auto grad = [&](float x) { return none ? 0.f : weight * exp_from<T>(x, top, neg, scale); };
+  auto grad = [&](float x) { return none ? 0.f : weight * exp_from(x, top, scale); };
   const bool same = (((uintptr_t)(z + first) ^ (uintptr_t)(out + first)) & 15) == 0;
   // where the two rows sit differently on their 16-byte lines, every element goes by itself
   const int64_t head = same ? min(last, first + (int64_t)((16 - ((uintptr_t)(z + first) & 15)) & 15) / (int64_t)sizeof(T)) : last;
@@ -367,7 +358,7 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const T* log
     if (ei[j] < 0) continue;
     float q = 0.f;  // all entries of this place, in order: equal indices write equal values
     for (int m = 0; m < e.k; ++m) q += ei[m] == ei[j] ? eq[m] : 0.f;
-    const float p = exp_from<T>(load1(z + first + ei[j]), top, neg, scale) / sum;
+    const float p = exp_from(load1(z + first + ei[j]), top, scale) / sum;
     out[first + ei[j]] = make1<T>(up * (p - q));
   }
 }

@@ -419,6 +419,25 @@ def test_distillation_same_index_twice_and_masked_values(cuda):
     assert l3[0] == math.inf and d3[0].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_distillation_rows_of_the_lowest_value(cuda, dtype):
+    """A row masked with its type's lowest value throughout is uniform; large logits lose nothing against their differences."""
+    z, i, s, up = make_kd(cuda, 6, 4003, 9, dtype, seed=11)
+    z[1] = torch.finfo(dtype).min
+    z[2, 100:] = torch.finfo(dtype).min
+    i[2] = torch.arange(9, device=cuda)
+    z[3] = (torch.randint(0, 8, (4003,), device=cuda) + 16000).to(dtype)   # whole numbers: exact in every type but bfloat16, where they are 16000 + 0 or 64
+    z[4] = -z[3]
+    for temperature in (1.0, 3.0):
+        rl, rz, p, q, _ = reference_kd(z, i, s, up, temperature)
+        loss, dz = step_kd(z, i, s, up, temperature)
+        # the tolerances of differences alone: they are at most 64 / T here, or the masked ones' exp is 0 on both sides
+        tol = temperature**2 * 2.0**-20 * (4 + (64 + 32) / temperature)
+        assert ((loss.double() - rl).abs() <= tol).all()
+        u = half_step(dtype)
+        assert ((dz.double() - rz).abs() <= u * rz.abs() + (p + q) * 2.0**-20 * (4 + 96 / temperature) + u * torch.finfo(dtype).tiny).all()
+
+
 def test_distillation_index_outside_the_vocabulary_is_nan(cuda):
     z, i, s, up = make_kd(cuda, 10, 5000, 6, torch.bfloat16)
     want = step_kd(z, i, s, up)
@@ -553,6 +572,32 @@ def test_another_stream_and_a_captured_step(cuda):
     graphs[0].replay()
     torch.cuda.synchronize()
     check_ce(x, w, t, up, *outs[0][:3])
+
+
+def test_the_first_calls_of_a_process_may_be_captured(cuda):
+    """Nothing has to run before a capture: no kernel needs a warm-up, nothing allocates outside ATen's pools."""
+    import subprocess
+    import sys
+    code = """
+import torch, tensorcomprehensions_b200 as tc
+x = torch.randn(40, 64, device="cuda").bfloat16().requires_grad_(); w = torch.randn(300, 64, device="cuda").bfloat16().requires_grad_()
+xf = torch.randn(2, 64, device="cuda").requires_grad_(); wf = torch.randn(300, 64, device="cuda")
+t = torch.randint(0, 300, (40,), device="cuda"); up = torch.rand(40, device="cuda")
+z = torch.randn(5, 4000, device="cuda").requires_grad_(); i = torch.randint(0, 4000, (5, 7), device="cuda"); s = torch.randn(5, 7, device="cuda"); uk = torch.rand(5, device="cuda")
+def step():
+    a = tc.linear_cross_entropy(x, w, t); b = tc.linear_cross_entropy(xf, wf, t[:2]); c = tc.topk_distillation(z, i, s)
+    return [a.detach(), b.detach(), c.detach(), *torch.autograd.grad(a, (x, w), up), *torch.autograd.grad(b, (xf,), up[:2]), *torch.autograd.grad(c, (z,), uk)]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = step()
+g.replay(); torch.cuda.synchronize()
+want = step(); torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, want))
+print("captured ok")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured ok" in r.stdout, r.stdout + r.stderr
 
 
 def test_the_same_bits_on_every_run(cuda):
