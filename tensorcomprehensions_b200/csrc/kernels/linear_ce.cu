@@ -623,8 +623,10 @@ int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
   const int64_t kb = ceil_div(l->bwd_piece, pg::kBK) * products;
   int64_t best = INT64_MAX;
   l->splits = 1;
-  // planes of at most 256 MiB
-  for (int64_t s = 1; s == 1 || (s <= 64 && s * 8 <= kb && s * l->n_pad * l->dp * 4 <= kPieceBytes); ++s) {
+  for (int64_t rounds = 0; rounds <= 7 && !l->few_bwd; ++rounds) {
+    const int64_t s = rounds ? rounds * pairs / tiles : 1;  // no split, or the splits that fill so many rounds
+    // planes of at most 256 MiB
+    if (s < 1 || s > 64 || (s > 1 && (s * 8 > kb || s * l->n_pad * l->dp * 4 > kPieceBytes))) continue;
     const int64_t cost = ceil_div(tiles * s, pairs) * (ceil_div(kb, s) + 8) + s * (9 * tiles / pairs + 1);
     if (cost < best) {
       best = cost;
