@@ -334,6 +334,7 @@ __device__ __forceinline__ void unscale(float (&acc)[C], const float* row_factor
 template <bool F32>
 struct ForwardEpi {
   static constexpr int kColumns = 128;
+  static constexpr bool kDirect = false;
   const Head* head;
   const int* target;
   float2* part;      // [parts][n_pad]
@@ -342,25 +343,34 @@ struct ForwardEpi {
   const float *row_factor, *col_factor;
   template <int C>
   __device__ void operator()(float (&acc)[C], int row, int col0, int, const CUtensorMap*, const pg::Out&) const {
-    if (row >= head->live || col0 >= v) return;
-    if (F32) unscale(acc, row_factor, col_factor, row, col0);
+    const bool live = row < head->live;
+    if (col0 >= v || !__any_sync(0xffffffffu, live)) return;
+    if (F32 && live) unscale(acc, row_factor, col_factor, row, col0);
     const int have = (int)min(v - col0, (int64_t)C);
-    const int64_t at = (int64_t)target[row] - v0 - col0;
+    const int64_t at = live ? (int64_t)target[row] - v0 - col0 : -1;
     const int t = at >= 0 && at < have ? (int)at : -1;
-    float top = -INFINITY, z = 0.f;
+    if (have < C) {  // the same for all lanes
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
-      if (j >= have) acc[j] = -INFINITY;
-      top = fmaxf(top, acc[j]);
-      if (j == t) z = acc[j];
+      for (int j = 0; j < C; ++j)
+        if (j >= have) acc[j] = -INFINITY;
     }
-    // all -inf: the sum is empty, and -inf - -inf would make NaN of it
-    const float shift = top == -INFINITY ? 0.f : top;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    if (__any_sync(0xffffffffu, t >= 0)) {  // rare: a warp's rows have their target in 32 x C of the logits
+      float z = 0.f;
 #pragma unroll
-    for (int j = 0; j < C; ++j) sum[j & 3] += exp_neg(acc[j] - shift);
-    part[(part0 + col0 / C) * n_pad + row] = make_float2(top, (sum[0] + sum[1]) + (sum[2] + sum[3]));
-    if (t >= 0) hit[row] = z;
+      for (int j = 0; j < C; ++j)
+        if (j == t) z = acc[j];
+      if (t >= 0) hit[row] = z;
+    }
+    float top = acc[0];
+#pragma unroll
+    for (int j = 1; j < C; ++j) top = fmaxf(top, acc[j]);
+    // all -inf: the sum is empty, and -inf - -inf would make NaN of it; all NaN: the sum says so
+    const float shift = top == -INFINITY || top != top ? 0.f : top;
+    const float2 neg = make_float2(-shift, -shift);
+    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+    for (int j = 0; j < C; j += 2) sum[(j >> 1) & 1] = __fadd2_rn(sum[(j >> 1) & 1], exp_neg2(make_float2(acc[j], acc[j + 1]), neg));
+    if (live) part[(part0 + col0 / C) * n_pad + row] = make_float2(top != top ? -INFINITY : top, (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
   }
 };
 
@@ -416,6 +426,7 @@ struct GradEpi {
   // three planes of a float32 value are five times the work of one rounding: sixteen warps of 64 columns
   // (1024 x 1024 x 16384: 120 -> 102 us), where 16-bit types lose by them (4096 x 2048 x 32000: 348 -> 361 us)
   static constexpr int kColumns = TYPE == kF32 ? 64 : 128;
+  static constexpr bool kDirect = TYPE != kF32;  // (float32 dZ above: 164k cycles without, 173k with)
   const Head* head;
   const int* target;
   const float* share;
@@ -430,12 +441,32 @@ struct GradEpi {
     const float g = live ? share[row] : 0.f, l = live ? lse[row] : 0.f;
     const int64_t at = live ? (int64_t)target[row] - v0 - col0 : -1;
     const int t = at >= 0 && at < C ? (int)at : -1;
-    const int have = live ? (int)min(v - col0, (int64_t)C) : 0;
+    const float2 neg = make_float2(-l, -l), g2 = make_float2(g, g);
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const float d = acc[c] - l;
-      const float p = TYPE == kF32 ? expf(d) : exp_neg(d);
-      acc[c] = c < have ? g * (c == t ? p - 1.f : p) : 0.f;
+    for (int c = 0; c < C; c += 2) {
+      float2 p;
+      if (TYPE == kF32) p = make_float2(expf(acc[c] - l), expf(acc[c + 1] - l));
+      else p = exp_neg2(make_float2(acc[c], acc[c + 1]), neg);
+      acc[c] = p.x;
+      acc[c + 1] = p.y;
+    }
+    if (__any_sync(0xffffffffu, t >= 0)) {  // rare, as in the forward pass
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (c == t) acc[c] -= 1.f;
+    }
+#pragma unroll
+    for (int c = 0; c < C; c += 2) {
+      const float2 x = __fmul2_rn(make_float2(acc[c], acc[c + 1]), g2);
+      acc[c] = x.x;
+      acc[c + 1] = x.y;
+    }
+    // rows behind the last live one, and what lies behind the vocabulary, are summed over by the products that follow: zero
+    const int have = live ? (int)min(v - col0, (int64_t)C) : 0;
+    if (__any_sync(0xffffffffu, have < C)) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (c >= have) acc[c] = 0.f;
     }
 #pragma unroll
     for (int p = 0; p < (TYPE == kF32 ? 3 : 1); ++p) {
@@ -468,6 +499,7 @@ struct GradEpi {
 // dX of a piece: fp32 sums, one plane per split of the piece, added to over the pieces.
 struct SumEpi {
   static constexpr int kColumns = 128;
+  static constexpr bool kDirect = false;
   int64_t ld;  // columns of the sums
   int add;
   template <int C>
@@ -490,6 +522,7 @@ struct SumEpi {
 template <typename T>
 struct WeightEpi {
   static constexpr int kColumns = 128;
+  static constexpr bool kDirect = false;
   const Head* head;
   T* dst;
   int64_t rows, d;
@@ -597,7 +630,7 @@ int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
   if (p.N > limit || p.V > limit || p.D > (1ll << 20) || p.ldw > (1ll << 38) || p.ldx > (1ll << 38)) return TCB200_ERR_TOO_LARGE;
   if (!pack_w(p) && p.ldw % 8 != 0) return TCB200_ERR_ALIGNMENT;
   l->n_pad = round_up(std::max<int64_t>(p.N, 1), kTile);
-  l->dp = round_up(p.D, 8);
+  l->dp = round_up(p.D, 64);  // packed rows start on 128-byte lines
   l->planes = p.dtype == TCB200_F32 ? 3 : 1;
   const int64_t v_pad = round_up(p.V, kTile);
   // A packed piece of W, and dZ of a piece, take at most 256 MiB where that leaves 4096 entries a piece; pieces are even.

@@ -40,8 +40,21 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { retur
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// exp(x), x <= 0: the base-2 exponential of the hardware; the product rounds x log2(e) to 2^-24 of itself
-__device__ __forceinline__ float exp_neg(float x) { return exp2f(x * kLog2e); }
+// exp(x), x <= 0: the base-2 exponential of the hardware (results below the smallest normal number become 0); the product
+// rounds x log2(e) to 2^-24 of itself
+__device__ __forceinline__ float exp_neg(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * kLog2e));
+  return y;
+}
+// two exp(x - shift): the packed fp32 instructions do the same arithmetic in half the issue slots
+__device__ __forceinline__ float2 exp_neg2(float2 x, float2 neg_shift) {
+  const float2 d = __fmul2_rn(__fadd2_rn(x, neg_shift), make_float2(kLog2e, kLog2e));
+  float2 y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(d.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(d.y));
+  return y;
+}
 
 // Running maximum and sum of exp(z - maximum).  An empty pair is (-inf, 0).
 struct Running {
