@@ -210,11 +210,17 @@ __global__ void __launch_bounds__(256) pack_kernel(const __half* in, int64_t ld,
 // tile, are zero.  Every block reads all targets (and all g, for the largest of them) and knows from them where its own
 // rows go: one launch instead of two that wait for one another, and the order of the live rows, and with it every later
 // sum, does not depend on timing.
+// It also settles how often the sum of dX is split: by the live rows, which the host does not know.
+struct Splits {
+  int64_t tiles;        // rows, in tiles, that the stack of partial sums has room for
+  int64_t tiles_n;      // tiles of a row of dX
+  int kb, products, pairs;
+};
 constexpr int kRowThreads = 512;
 template <typename T, typename Index>
 __global__ void __launch_bounds__(kRowThreads) rows_kernel(const Index* target, int64_t n, int64_t v, int64_t ignore,
                                                            const float* g, int64_t g_stride, const float* lse, Rows r,
-                                                           const T* x, int64_t ld, int64_t d, int64_t dp, Planes o) {
+                                                           const T* x, int64_t ld, int64_t d, int64_t dp, Planes o, Splits sp) {
   __shared__ int before_of[kRowThreads / 32], all_of[kRowThreads / 32];
   __shared__ float top_of[kRowThreads / 32];
   __shared__ int list[kRowThreads];
@@ -255,6 +261,10 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const Index* target, 
     r.head->live = all;
     r.head->status = 0;
     r.head->gscale = top > 0.f ? top : 1.f;
+    const int64_t tiles_m = (all + (int64_t)kTile - 1) / kTile, tiles = tiles_m * sp.tiles_n;
+    r.head->splits = tiles == 0 || tiles > 1 << 20
+                         ? 1
+                         : pg::choose_splits((int)tiles, sp.kb, sp.products, sp.pairs, (int)min(sp.tiles / tiles_m, (int64_t)pg::kMaxSplits));
   }
   const uint32_t per_row = (uint32_t)(dp / 8);
   // 512 rows at a time: their places, then their X
@@ -496,14 +506,16 @@ struct GradEpi {
   }
 };
 
-// dX of a piece: fp32 sums, one plane per split of the piece, added to over the pieces.
+// dX of a piece: fp32 sums, a stack of partial ones where the vocabulary is split, added to over the pieces.
 struct SumEpi {
   static constexpr int kColumns = 128;
   static constexpr bool kDirect = false;
+  const Head* head;
   int64_t ld;  // columns of the sums
   int add;
   template <int C>
   __device__ void operator()(float (&acc)[C], int row, int col0, int split, const CUtensorMap* tm, const pg::Out& out) const {
+    const int at = row - out.lane + split * ((head->live + kTile - 1) / kTile * kTile);
 #pragma unroll
     for (int h = 0; h < C; h += 32) {
       if (col0 + h >= ld) return;
@@ -512,8 +524,8 @@ struct SumEpi {
       for (int c = 0; c < 32; c += 4)
         out.put(c / 4, make_uint4(__float_as_uint(acc[h + c]), __float_as_uint(acc[h + c + 1]), __float_as_uint(acc[h + c + 2]),
                                   __float_as_uint(acc[h + c + 3])));
-      if (add) out.send_add(tm, col0 + h, row - out.lane, split);
-      else out.send(tm, col0 + h, row - out.lane, split);
+      if (add) out.send_add(tm, col0 + h, at, 0);
+      else out.send(tm, col0 + h, at, 0);
     }
   }
 };
@@ -563,7 +575,7 @@ struct WeightEpi {
 
 // dX: the splits' sums added in order, scaled, rounded once and put back in the rows' places; zero where a row has no target.
 template <typename T>
-__global__ void __launch_bounds__(256) finish_kernel(Rows r, const float* sums, int splits, int64_t plane, int64_t ld,
+__global__ void __launch_bounds__(256) finish_kernel(Rows r, const float* sums, int64_t ld,
                                                      int64_t n, int64_t d, float scale, T* dx, T* dw,
                                                      int* dev_status) {
   pdl_sync();
@@ -573,6 +585,8 @@ __global__ void __launch_bounds__(256) finish_kernel(Rows r, const float* sums, 
   if (bad && dw && blockIdx.x == 0 && threadIdx.x == 0) dw[0] = from_float<T>(nan);
   if (!dx) return;
   const float k = r.head->gscale * scale;
+  const int splits = r.head->splits;
+  const int64_t plane = ((int64_t)r.head->live + kTile - 1) / kTile * kTile * ld;
   const int64_t per_row = ld / 8;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n * per_row; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t row = i / per_row, c = (i % per_row) * 8;
@@ -610,7 +624,7 @@ struct Layout {
   int64_t fwd_piece, bwd_piece;  // vocabulary entries per piece
   int64_t parts;                 // of a row's logits, one per drain warp's columns
   int fwd_bn, bwd_bn, dw_bn;     // columns of a tile: logits forward, logits backward, dW
-  int splits;                    // planes of partial sums of dX
+  int splits, split_for;         // partial sums of dX that there is room for; k-blocks that their number is chosen for
   bool few_fwd, few_bwd;         // the kernels for few rows: nothing is packed, no dZ is kept
   int64_t fwd_bytes, bwd_bytes;
   // byte offsets
@@ -649,23 +663,12 @@ int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
   l->few_fwd = few_forward_ok(p);
   l->few_bwd = few_backward_ok(p);
   l->parts = l->few_fwd ? few_blocks(p, sms, false) : ceil_div(p.V, l->fwd_bn / 2);
-  // dX has few tiles and a long sum: the vocabulary of a piece is split where that fills the last round of the pairs.
-  // Cost of S splits in k-blocks of a pair: rounds x (a unit's k-blocks + 8 for its start and epilogue) + what adding S
-  // planes costs (a plane of a tile is about 4 k-blocks of memory traffic).
-  const int64_t tiles = (l->n_pad / kTile) * ceil_div(p.D, kTile), pairs = std::max(1, sms / 2);
-  const int64_t kb = ceil_div(l->bwd_piece, pg::kBK) * products;
-  int64_t best = INT64_MAX;
-  l->splits = 1;
-  for (int64_t rounds = 0; rounds <= 7 && !l->few_bwd; ++rounds) {
-    const int64_t s = rounds ? rounds * pairs / tiles : 1;  // no split, or the splits that fill so many rounds
-    // planes of at most 256 MiB
-    if (s < 1 || s > 64 || (s > 1 && (s * 8 > kb || s * l->n_pad * l->dp * 4 > kPieceBytes))) continue;
-    const int64_t cost = ceil_div(tiles * s, pairs) * (ceil_div(kb, s) + 8) + s * (9 * tiles / pairs + 1);
-    if (cost < best) {
-      best = cost;
-      l->splits = (int)s;
-    }
-  }
+  // dX has few tiles and a long sum, which is split (pg::choose_splits) by the live rows; there is room for the partial sums of
+  // all rows, 256 MiB of them at most.
+  const int64_t tiles = (l->n_pad / kTile) * ceil_div(p.D, kTile);
+  l->split_for = (int)ceil_div(l->bwd_piece, pg::kBK);
+  l->splits = tiles > 1 << 20 ? 1 : pg::choose_splits((int)tiles, l->split_for, products, std::max(1, sms / 2),
+                                                      (int)std::max<int64_t>(1, std::min<int64_t>(pg::kMaxSplits, kPieceBytes / (l->n_pad * l->dp * 4))));
   if (l->few_bwd) l->splits = (int)few_blocks(p, sms, true);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -720,7 +723,9 @@ int launch_rows_typed(const tcb200_linear_ce_t& p, const Layout& l, const void* 
   // blocks enough for the rows' copies, zero rows of the last tile among them
   const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(l.n_pad * (l.dp / 8), kRowThreads), 2ll * sms);
   TCB200_CUDA_TRY(launch_pdl(rows_kernel<T, Index>, dim3(blocks), dim3(kRowThreads), 0, s, static_cast<const Index*>(target),
-                             p.N, p.V, p.ignore_index, g, g_stride, lse, r, static_cast<const T*>(X), p.ldx, p.D, l.dp, o));
+                             p.N, p.V, p.ignore_index, g, g_stride, lse, r, static_cast<const T*>(X), p.ldx, p.D, l.dp, o,
+                             Splits{l.splits * (l.n_pad / kTile), ceil_div(p.D, kTile), l.split_for,
+                                    l.planes == 3 ? 6 : 1, std::max(1, sms / 2)}));
   return TCB200_OK;
 }
 // f16 and bf16 are copied as they are
@@ -761,7 +766,6 @@ pg::Args gemm_args(int64_t M, int64_t N, int64_t K, const int* live, int live_is
   // in the end take 1024 k: half as many drains, which leaves the epilogues twice the time before they hold up the MMAs
   // (dZ of 4096 x 2048 x 32000: 414 -> 350 us).
   a.chunk_kb = products > 1 ? 4 : forward ? 8 : 16;
-  a.splits = 1;
   a.dev_status = status;
   return a;
 }
@@ -811,12 +815,11 @@ int backward_typed(const tcb200_linear_ce_t& p, const Layout& l, const void* W, 
     if (st != TCB200_OK) return st;
     const pg::Operand z{dz, v, l.n_pad, ld, l.planes, l.n_pad * ld};
     if (dX) {
-      const SumEpi se{l.dp, v0 > 0};
-      st = pg::make_out_map(&tc, {sums, l.dp, l.n_pad, l.dp, l.splits, l.n_pad * l.dp}, 4);
+      const SumEpi se{r.head, l.dp, v0 > 0};
+      st = pg::make_out_map(&tc, {sums, l.dp, l.splits * l.n_pad, l.dp, 1, 0}, 4);
       if (st != TCB200_OK) return st;
       pg::Args a = gemm_args(p.N, p.D, v, live, 0, status, products, false);
-      a.splits = l.splits;
-      a.split_kb = (int)ceil_div(ceil_div(v, pg::kBK), l.splits);
+      a.splits = &r.head->splits;
       if ((st = pg::launch<256, false, true>(z, w, bf16, a, tc, se, device, sms, s)) != TCB200_OK) return st;
     }
     if (dW) {
@@ -830,8 +833,7 @@ int backward_typed(const tcb200_linear_ce_t& p, const Layout& l, const void* W, 
     }
   }
   const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(p.N * (l.dp / 8), 256), 8ll * sms)));
-  TCB200_CUDA_TRY(launch_pdl(finish_kernel<T>, grid, dim3(256), 0, s, r, static_cast<const float*>(sums), l.splits,
-                             l.n_pad * l.dp, l.dp, p.N, p.D, scale, dX, dW, dev_status));
+  TCB200_CUDA_TRY(launch_pdl(finish_kernel<T>, grid, dim3(256), 0, s, r, static_cast<const float*>(sums), l.dp, p.N, p.D, scale, dX, dW, dev_status));
   return TCB200_OK;
 }
 

@@ -15,6 +15,7 @@ struct Head {
   int live;      // rows with a target
   int status;    // a bounded wait that gave up
   float gscale;  // largest |g| of the live rows
+  int splits;    // partial sums of dX
 };
 
 struct Rows {

@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NR)) few_forward_kerne
     const int64_t t = f.index(threadIdx.x);
     rows.place[threadIdx.x] = t != f.ignore ? (int)threadIdx.x : -1;
     rows.target[threadIdx.x] = t >= 0 && t < f.v ? (int)t : -1;
-    if (threadIdx.x == 0) *rows.head = Head{(int)f.n, 0, 1.f};
+    if (threadIdx.x == 0) *rows.head = Head{(int)f.n, 0, 1.f, 1};
   }
   const int value = lane / SHARE, r = value / PER, e = value % PER;
   const int64_t t = r < f.n ? f.index(r) : -1;
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1) few_ring_kernel(const __grid
     const int64_t t = f.index(threadIdx.x);
     rows.place[threadIdx.x] = t != f.ignore ? (int)threadIdx.x : -1;
     rows.target[threadIdx.x] = t >= 0 && t < f.v ? (int)t : -1;
-    if (threadIdx.x == 0) *rows.head = Head{(int)f.n, 0, 1.f};
+    if (threadIdx.x == 0) *rows.head = Head{(int)f.n, 0, 1.f, 1};
   }
   int* status = &rows.head->status;
   const int groups = (int)((f.v + kBoxRows - 1) / kBoxRows), chunks = (int)((f.d + CHUNK - 1) / CHUNK);
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, NR <= 2 ? 2 : 1) few_backward_kernel
   for (int i = threadIdx.x; i < NR * dp; i += kThreads) sdx[i] = 0.f;
   if (blockIdx.x == 0 && threadIdx.x < f.n) {
     rows.place[threadIdx.x] = f.index(threadIdx.x) != f.ignore ? (int)threadIdx.x : -1;
-    if (threadIdx.x == 0) *rows.head = Head{(int)f.n, 0, 1.f};
+    if (threadIdx.x == 0) *rows.head = Head{(int)f.n, 0, 1.f, 1};
   }
   const int value = lane / SHARE, r = value / PER, e = value % PER;
   const int64_t t = r < f.n ? f.index(r) : f.ignore;

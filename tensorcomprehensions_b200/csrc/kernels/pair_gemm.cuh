@@ -49,7 +49,7 @@ struct Args {
   int products;             // plane products per k-block: 1, or 3 or 6 for float32
   int pa[kMaxProducts], pb[kMaxProducts];
   int chunk_kb;             // k-blocks per drain
-  int splits, split_kb;     // the reduction's k-blocks go to `splits` units of split_kb each
+  const int* splits;        // null, or a device count of units that the reduction of a tile is split over
   uint32_t idesc;           // instruction descriptor
   int* dev_status;
 };
@@ -115,6 +115,29 @@ __device__ __forceinline__ void load_operand(uint8_t* dst, const CUtensorMap* tm
   }
 }
 
+// Splits of a reduction over `kb` k-blocks of `products` plane products whose result has `tiles` tiles, at most `most`: the number
+// that ends first on `pairs` pairs.  In k-blocks of a pair: rounds x (a unit's k-blocks + 8 for its start and epilogue) + what
+// adding the partial sums costs (writing and reading a tile of one takes about 9).  Candidates are one, and what fills whole
+// rounds with units of eight k-blocks and more.
+__host__ __device__ inline int choose_splits(int tiles, int kb, int products, int pairs, int most) {
+  const int steps = kb * products, shortest = steps / 8 < kb ? steps / 8 : kb;
+  if (most > shortest) most = shortest;
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int rounds = 0; rounds <= 7; ++rounds) {
+    int s = rounds ? (int)((int64_t)rounds * pairs / tiles) : 1;
+    if (s > most) s = most;
+    if (s < 1) continue;
+    const int64_t cost = (int64_t)((tiles * s + pairs - 1) / pairs) * ((steps + s - 1) / s + 8) + (int64_t)s * (9 * tiles / pairs + 1);
+    if (cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+constexpr int kMaxSplits = 64;
+
 // A unit is (tile, split).  Tiles are taken in groups of 8 tile rows, rows fastest inside a group: the pairs that run at the
 // same time then share rows of B (8 pairs each) and of A, which the L2 serves.
 struct Units {
@@ -126,8 +149,8 @@ struct Units {
     tiles_m = (M + kTile - 1) / kTile;
     tiles_n = (a.N + bn - 1) / bn;
     kb = (int)((K + kBK - 1) / kBK);
-    splits = a.splits;
-    split_kb = a.split_kb > 0 ? a.split_kb : kb;
+    splits = a.splits ? *a.splits : 1;
+    split_kb = (kb + splits - 1) / splits;
     units = tiles_m * tiles_n * splits;
   }
   __device__ void locate(int64_t u, int64_t* tm, int64_t* tn, int* split, int* kb0, int* nkb) const {
@@ -409,9 +432,10 @@ int launch(const Operand& A, const Operand& B, bool bf16, Args args, const CUten
     args.pa[i] = pa[6 - args.products + i];
     args.pb[i] = pb[6 - args.products + i];
   }
-  const int64_t units = ceil_div(args.M, kTile) * ceil_div(args.N, BN) * args.splits;
-  if (units == 0) return TCB200_OK;
-  const unsigned pairs = (unsigned)std::min<int64_t>(units, std::max(1, sms / 2));
+  const int64_t tiles = ceil_div(args.M, kTile) * ceil_div(args.N, BN);
+  if (tiles == 0) return TCB200_OK;
+  // (a split result takes all pairs: how many units there are only the kernel knows)
+  const unsigned pairs = (unsigned)std::min<int64_t>(args.splits ? INT64_MAX : tiles, std::max(1, sms / 2));
   static std::atomic<uint64_t> configured{0};
   TCB200_CUDA_TRY(ensure_dynamic_smem(pair_gemm_kernel<BN, C, A_MN, B_MN, Epi>, BYTES, device, configured));
   TCB200_CUDA_TRY(launch_pdl(pair_gemm_kernel<BN, C, A_MN, B_MN, Epi>, dim3(2 * pairs), dim3(block_threads(BN, C)), BYTES, s, ta, tb, tc, args, epi));
