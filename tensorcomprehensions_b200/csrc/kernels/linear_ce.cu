@@ -144,22 +144,39 @@ struct Planes {
   int64_t stride;  // elements from one plane to the next
 };
 
-// A warp packs a row of float32 (source null: a row of zeros).
-__device__ __forceinline__ void pack_row(const float* src, int64_t d, int64_t dp, const Planes& o, int64_t row) {
-  const int lane = threadIdx.x & 31;
+// L lanes (a warp, or half or a quarter of one where rows are short) pack a row of float32; source null: a row of zeros;
+// `write` false: nothing (the lanes take part in the shuffles all the same).  Rows of up to 16 L columns stay in registers
+// between finding their largest value and writing; longer ones are read again.
+template <int L>
+__device__ __forceinline__ void pack_row(const float* src, bool write, int64_t d, int64_t dp, const Planes& o, int64_t row) {
+  constexpr int SPAN = L * 8, HOLD = 2;
+  const int lane = threadIdx.x & (L - 1);
+  auto load = [&](int64_t c0, float* v) {
+    if (src && c0 + lane * 8 < d) load8(src + c0 + lane * 8, d - c0 - lane * 8, v);
+    else memset(v, 0, 32);
+  };
   float top = 0.f;
-  if (src)
-#pragma unroll 2
-    for (int64_t c = lane * 8; c < d; c += 256) {
-      alignas(16) float v[8];
-      load8(src + c, d - c, v);
+  auto look = [&](const float* v) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float a = fabsf(v[j]);
-        if (a <= kLargest) top = fmaxf(top, a);
-      }
+    for (int j = 0; j < 8; ++j) {
+      const float a = fabsf(v[j]);
+      if (a <= kLargest) top = fmaxf(top, a);
     }
-  for (int q = 16; q; q >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, q));
+  };
+  alignas(16) float held[HOLD][8];
+#pragma unroll
+  for (int h = 0; h < HOLD; ++h)
+    if (h * SPAN < dp) load(h * SPAN, held[h]);
+#pragma unroll
+  for (int h = 0; h < HOLD; ++h)
+    if (h * SPAN < dp) look(held[h]);
+  for (int64_t c0 = HOLD * SPAN; c0 < d; c0 += SPAN) {
+    alignas(16) float v[8];
+    load(c0, v);
+    look(v);
+  }
+#pragma unroll
+  for (int q = L / 2; q; q >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, q));
   int e = 0;
   if (top > 0.f) {
     frexpf(top, &e);
@@ -167,11 +184,9 @@ __device__ __forceinline__ void pack_row(const float* src, int64_t d, int64_t dp
   }
   e = min(e, 126);  // (the smallest e is -113; both 2^e and 2^-e are normal numbers)
   const float scale = ldexpf(1.f, e);
-  if (lane == 0) o.factor[row] = ldexpf(1.f, -e);
-#pragma unroll 2
-  for (int64_t c = lane * 8; c < dp; c += 256) {
-    alignas(16) float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (src) load8(src + c, d - c, v);
+  if (lane == 0 && write) o.factor[row] = ldexpf(1.f, -e);
+  auto emit = [&](int64_t c, const float* v) {
+    if (!write || c >= dp) return;
     alignas(16) uint16_t h[2][8], p[3][8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -186,13 +201,40 @@ __device__ __forceinline__ void pack_row(const float* src, int64_t d, int64_t dp
     if (o.plain)
 #pragma unroll
       for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(o.plain + k * o.stride + row * dp + c) = *reinterpret_cast<uint4*>(p[k]);
+  };
+#pragma unroll
+  for (int h = 0; h < HOLD; ++h)
+    if (h * SPAN < dp) emit(h * SPAN + lane * 8, held[h]);
+  for (int64_t c0 = HOLD * SPAN; c0 < dp; c0 += SPAN) {
+    alignas(16) float v[8];
+    load(c0, v);
+    emit(c0 + lane * 8, v);
   }
+}
+// Rows first, first + stride, ... below `rows` of a warp; source(r) is their address or null.
+template <int L, typename Source>
+__device__ __forceinline__ void pack_rows_of(int64_t first, int64_t stride, int64_t rows, int64_t d, int64_t dp, const Planes& o, int64_t row0,
+                                             Source source) {
+  constexpr int PER = 32 / L;
+  const int mine = (threadIdx.x & 31) / L;
+  for (int64_t r = first * PER; r < rows; r += stride * PER) {
+    const bool there = r + mine < rows;
+    pack_row<L>(there ? source(r + mine) : nullptr, there, d, dp, o, row0 + r + mine);
+  }
+}
+template <typename Source>
+__device__ __forceinline__ void pack_rows(int64_t first, int64_t stride, int64_t rows, int64_t d, int64_t dp, const Planes& o, int64_t row0,
+                                          Source source) {
+  if (dp <= 64) pack_rows_of<8>(first, stride, rows, d, dp, o, row0, source);
+  else if (dp <= 128) pack_rows_of<16>(first, stride, rows, d, dp, o, row0, source);
+  else pack_rows_of<32>(first, stride, rows, d, dp, o, row0, source);
 }
 
 // Entries of W as operand planes of [rows][dp], dp = d rounded up to 8.
 __global__ void __launch_bounds__(256) pack_rows_kernel(const float* in, int64_t ld, int64_t rows, int64_t d, int64_t dp, Planes o) {
   pdl_sync();
-  for (int64_t r = blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8) pack_row(in + r * ld, d, dp, o, r);
+  const int warp = threadIdx.x >> 5;
+  pack_rows(blockIdx.x * 8 + warp, gridDim.x * 8, rows, d, dp, o, 0, [&](int64_t r) { return in + r * ld; });
 }
 __global__ void __launch_bounds__(256) pack_kernel(const __half* in, int64_t ld, int64_t rows, int64_t d, int64_t dp, Planes o) {
   pdl_sync();
@@ -218,7 +260,7 @@ struct Splits {
 };
 constexpr int kRowThreads = 512;
 template <typename T, typename Index>
-__global__ void __launch_bounds__(kRowThreads) rows_kernel(const Index* target, int64_t n, int64_t v, int64_t ignore,
+__global__ void __launch_bounds__(kRowThreads, 2) rows_kernel(const Index* target, int64_t n, int64_t v, int64_t ignore,
                                                            const float* g, int64_t g_stride, const float* lse, Rows r,
                                                            const T* x, int64_t ld, int64_t d, int64_t dp, Planes o, Splits sp) {
   __shared__ int before_of[kRowThreads / 32], all_of[kRowThreads / 32];
@@ -296,7 +338,7 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const Index* target, 
     }
     __syncthreads();
     if constexpr (sizeof(T) == 4) {
-      for (int j = warp; j < count; j += kRowThreads / 32) pack_row(x + (base + list[j]) * ld, d, dp, o, before + j);
+      pack_rows(warp, kRowThreads / 32, count, d, dp, o, before, [&](int64_t j) { return x + (base + list[j]) * ld; });
     } else {
       const uint32_t items = (uint32_t)count * per_row;
       constexpr int U = 4;  // loads in flight a thread
@@ -320,8 +362,8 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const Index* target, 
   }
   const int64_t end = (all + (int64_t)kTile - 1) / kTile * kTile;
   if constexpr (sizeof(T) == 4) {
-    for (int64_t r = all + blockIdx.x * (kRowThreads / 32) + warp; r < end; r += gridDim.x * (kRowThreads / 32))
-      pack_row(nullptr, d, dp, o, r);
+    pack_rows(blockIdx.x * (kRowThreads / 32) + warp, gridDim.x * (kRowThreads / 32), end - all, d, dp, o, all,
+              [](int64_t) { return (const float*)nullptr; });
   } else {
     for (int64_t k = blockIdx.x * (int64_t)kRowThreads + threadIdx.x; k < (end - all) * per_row; k += (int64_t)gridDim.x * kRowThreads)
       *reinterpret_cast<uint4*>(o.plain + all * dp + k * 8) = make_uint4(0, 0, 0, 0);
