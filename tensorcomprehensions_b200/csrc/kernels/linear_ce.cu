@@ -727,7 +727,7 @@ int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
   const int64_t x_plane = l->few_fwd && l->few_bwd ? 0 : l->n_pad * l->dp * 2;
   l->x_factor = take(f32 ? l->n_pad * 4 : 0);
   l->x_scaled = take(f32 ? 2 * x_plane : 0);
-  l->x = f32 ? -1 : take(x_plane);
+  if (!f32) l->x = take(x_plane);
   const int64_t common = at;
   l->hit = take(l->n_pad * 4);
   l->part = take(l->parts * l->n_pad * 8);
@@ -737,7 +737,7 @@ int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
   l->w_fwd_factor = take(f32 ? l->fwd_piece * 4 : 0);
   l->fwd_bytes = at;
   at = common;
-  if (f32) l->x = take(3 * x_plane);
+  if (f32) l->x = take(3 * x_plane);  // (backward only)
   const int64_t bwd_plane = pack_w(p) && !l->few_bwd ? l->bwd_piece * l->dp * 2 : 0;
   l->w_bwd = take(l->planes * bwd_plane);
   l->w_bwd_scaled = take(f32 ? 2 * bwd_plane : 0);
@@ -773,7 +773,7 @@ int launch_rows_typed(const tcb200_linear_ce_t& p, const Layout& l, const void* 
 // f16 and bf16 are copied as they are
 int launch_rows(const tcb200_linear_ce_t& p, const Layout& l, const void* X, const void* target, const float* g,
                 int64_t g_stride, const float* lse, const Rows& r, char* ws, int sms, cudaStream_t s) {
-  Planes o{l.x < 0 || (p.dtype == TCB200_F32 && !g) ? nullptr : reinterpret_cast<uint16_t*>(ws + l.x), reinterpret_cast<uint16_t*>(ws + l.x_scaled),
+  Planes o{p.dtype == TCB200_F32 && !g ? nullptr : reinterpret_cast<uint16_t*>(ws + l.x), reinterpret_cast<uint16_t*>(ws + l.x_scaled),
            reinterpret_cast<float*>(ws + l.x_factor), l.n_pad * l.dp};
   const bool f32 = p.dtype == TCB200_F32, wide = p.index_bytes == 8;
   auto fn = f32 ? (wide ? launch_rows_typed<float, int64_t> : launch_rows_typed<float, int32_t>)

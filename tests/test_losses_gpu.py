@@ -82,7 +82,8 @@ def step_ce(x, w, t, up, **kw):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,d,v,ignored", [
     (1, 64, 256, 0), (1, 1, 1, 0), (1, 8, 2, 0), (3, 7, 5, 0), (2, 1000, 300, 0), (130, 65, 257, 0.3), (128, 64, 128, 0), (256, 256, 512, 0),
-    (257, 513, 1000, 0.2), (300, 136, 5000, 0.5), (64, 520, 1003, 0), (515, 24, 777, 0.9), (40, 2056, 640, 0)])
+    (257, 513, 1000, 0.2), (300, 136, 5000, 0.5), (64, 520, 1003, 0), (515, 24, 777, 0.9), (40, 2056, 640, 0),
+    (140, 112, 300, 0.1), (140, 60, 300, 0), (140, 700, 300, 0), (140, 1100, 300, 0), (2000, 256, 6000, 0.97), (1500, 512, 9000, 0.5), (1000, 1032, 2000, 0.1)])
 def test_linear_cross_entropy(cuda, dtype, n, d, v, ignored):
     x, w, t, up = make_ce(cuda, n, d, v, dtype, ignored, seed=n + d + v)
     check_ce(x, w, t, up, *step_ce(x, w, t, up))
