@@ -3,7 +3,8 @@
 //   q = softmax(teacher / T) over a row's K entries,  p = softmax(logits / T) over V
 //   loss = T^2 sum_k q_k (ln q_k - ln p_{i_k}),  dlogits_v = T g (p_v - sum_{k: i_k = v} q_k)
 //
-// Both directions are one pass over [N, V] and bound by HBM: forward reads it, backward reads it and writes as much.
+// Both directions are one pass over [N, V] and bound by HBM: forward reads it, backward reads it and writes as much
+// (4096 x 131072 bf16: 169 us, 6.4 TB/s, and 340 us, 6.3 TB/s).
 //
 // Forward: a cluster of CTAs takes a row (one CTA where the rows alone fill the device, up to eight where there are few), each
 // thread keeps the running maximum and sum of its elements, the CTAs' pairs meet in the first CTA's shared memory.  The
@@ -41,7 +42,7 @@ __device__ __forceinline__ uint4 load_raw(const void* p) {
   return v;
 }
 __device__ __forceinline__ void store_raw(void* p, const uint4& v) {
-  asm volatile("st.global.cs.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+  asm volatile("st.global.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 // base-2 exponential; results below the smallest normal number become 0
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -407,6 +408,7 @@ int backward_typed(const tcb200_topk_distill_t& p, const void* logits, const Ent
                    int64_t g_stride, void* dlogits, cudaStream_t s) {
   const int sms = sm_count(-1);
   // stretches of at most 32768 elements, and of 2048 and more while the rows make fewer than eight CTAs an SM
+  // (4096 x 131072 bf16, stretches of 8192 / 32768 / 65536 / 131072: 407 / 340 / 356 / 361 us)
   const int64_t fill = std::min<int64_t>(8ll * sms / p.N, p.V / 2048);
   const int parts = (int)std::max<int64_t>({1, fill, ceil_div(p.V, 32768)});
   TCB200_CUDA_TRY(launch_pdl(distill_backward_kernel<T>, dim3((unsigned)(p.N * parts)), dim3(kThreads), (size_t)p.K * 8, s,
