@@ -9,8 +9,10 @@
 // Forward: a cluster of CTAs takes a row (one CTA where the rows alone fill the device, up to eight where there are few), each
 // thread keeps the running maximum and sum of its elements, the CTAs' pairs meet in the first CTA's shared memory.  The
 // K entries are fetched before the pass over the row, so their latency hides behind it.
-// Backward: the row's maximum and sum are known, so a CTA takes any stretch of a row: it writes T g p for all of it, then, behind a block barrier,
-// writes the entries' places again with q taken off.  p - q is formed in fp32 and rounded once.
+// Backward: the row's maximum and sum are known, so a CTA takes any stretch of a row: it writes T g p for all of it, then, behind
+// a block barrier, writes the entries' places again with q taken off.  Equal indices are found by marking places in a bitmap;
+// only they are compared with all entries (100 x 32000 f16, K = 4000, both directions: 4.1 ms with every entry compared, 69 us
+// marked).  p - q is formed in fp32 and rounded once.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
@@ -21,7 +23,6 @@
 namespace tcb200 {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T> __device__ __forceinline__ float load1(const T* p);
@@ -185,6 +186,7 @@ __device__ __forceinline__ Running warp_join(Running r, float scale) {
   return r;
 }
 // All threads get the block's pairs (two at once); `share` holds two pairs a warp.  Pairs are joined in a fixed order.
+template <int kThreads>
 __device__ __forceinline__ void block_join(Running& a, Running& b, float scale, float4* share) {
   a = warp_join(a, scale);
   b = warp_join(b, scale);
@@ -208,7 +210,7 @@ __device__ __forceinline__ void stretch(int64_t v, int i, int n, int64_t* first,
 
 constexpr int kMaxCluster = 8;
 
-template <typename T>
+template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads) distill_forward_kernel(const T* logits, int64_t ld, int64_t v, Entries e,
                                                                    float temperature, float* loss, float* stats, int parts) {
   __shared__ float4 share[kThreads / 32];
@@ -257,7 +259,7 @@ __global__ void __launch_bounds__(kThreads) distill_forward_kernel(const T* logi
       bad |= at >= v;
       if (at >= 0) t.one(e.logit(row, j), scale);
     }
-  block_join(r, t, scale, share);
+  block_join<kThreads>(r, t, scale, share);
   if (parts > 1) {
     if (threadIdx.x == 0) {
       uint32_t at;
@@ -296,11 +298,12 @@ __global__ void __launch_bounds__(kThreads) distill_forward_kernel(const T* logi
   }
 }
 
-template <typename T>
+template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const T* logits, int64_t ld, int64_t v, Entries e,
                                                                     float temperature, const float* stats, const float* g,
                                                                     int64_t g_stride, T* dlogits, int parts) {
-  extern __shared__ float entry_mem[];  // q of the entries of this stretch, then their places in it (-1: none)
+  // q of the entries of this stretch, their places in it (-1: none), two bits a place: taken by an entry, by more than one
+  extern __shared__ float entry_mem[];
   pdl_sync();
   const int64_t row = blockIdx.x / parts;
   int64_t first, last;
@@ -309,6 +312,9 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const T* log
   T* out = dlogits + row * v;
   float* eq = entry_mem;
   int* ei = reinterpret_cast<int*>(entry_mem + e.k);
+  uint32_t* taken = reinterpret_cast<uint32_t*>(ei + e.k);
+  const int words = (int)((last - first + 31) / 32);
+  for (int j = threadIdx.x; j < 2 * words; j += kThreads) taken[j] = 0;  // (used behind the first barrier)
   const float inv = 1.f / temperature, scale = kLog2e * inv;
   const float top = stats[3 * row], sum = stats[3 * row + 1], log_weight = stats[3 * row + 2];
   const bool none = log_weight == -INFINITY;
@@ -357,8 +363,17 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const T* log
   __syncthreads();  // the entries' places are written again behind this
   for (int j = threadIdx.x; j < e.k; j += kThreads) {
     if (ei[j] < 0) continue;
-    float q = 0.f;  // all entries of this place, in order: equal indices write equal values
-    for (int m = 0; m < e.k; ++m) q += ei[m] == ei[j] ? eq[m] : 0.f;
+    const uint32_t bit = 1u << (ei[j] & 31);
+    if (atomicOr(&taken[ei[j] >> 5], bit) & bit) atomicOr(&taken[words + (ei[j] >> 5)], bit);
+  }
+  __syncthreads();
+  for (int j = threadIdx.x; j < e.k; j += kThreads) {
+    if (ei[j] < 0) continue;
+    float q = eq[j];
+    if (taken[words + (ei[j] >> 5)] >> (ei[j] & 31) & 1) {
+      q = 0.f;  // all entries of this place, in order: equal indices write equal values
+      for (int m = 0; m < e.k; ++m) q += ei[m] == ei[j] ? eq[m] : 0.f;
+    }
     const float p = exp_from(load1(z + first + ei[j]), top, scale) / sum;
     out[first + ei[j]] = make1<T>(up * (p - q));
   }
@@ -379,6 +394,15 @@ Entries entries_of(const tcb200_topk_distill_t& p, const void* indices, const vo
   return {indices, teacher, p.ld_indices, p.ld_teacher, (int)p.K, p.index_bytes, p.teacher_dtype};
 }
 
+// Threads of a CTA.  A short row is bound by its chain of loads and joins, not by its bytes: where the rows alone fill the device,
+// two warps a row keep four times as many rows in flight as eight do (8192 x 600 f16, K = 20: 32 -> 13 us forward, 23 -> 12 us
+// backward; 4096 x 8000 bf16, K = 50: 28 -> 20 and 28 -> 24).  Rows of 32 KB are better off with eight (4096 x 8000 f32 backward:
+// 58 -> 53 us), and so are many entries (8192 x 600 f16, K = 250 forward: 59 -> 47 us).
+int threads_for(const tcb200_topk_distill_t& p, int sms) {
+  const int64_t row = p.V * (p.logits_dtype == TCB200_F32 ? 4 : 2);
+  return p.N >= 8ll * sms && row <= 16384 && p.K <= 128 ? 64 : 256;
+}
+
 template <typename T>
 int forward_typed(const tcb200_topk_distill_t& p, const void* logits, const Entries& e, float* loss, float* stats,
                   cudaStream_t s) {
@@ -387,8 +411,9 @@ int forward_typed(const tcb200_topk_distill_t& p, const void* logits, const Entr
   int parts = 1;
   while (parts < kMaxCluster && p.N * parts < 8ll * sms && p.V / (parts * 2) >= 2048) parts *= 2;
   cudaLaunchConfig_t cfg = {};
+  const int threads = threads_for(p, sms);
   cfg.gridDim = dim3((unsigned)(p.N * parts));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -397,8 +422,9 @@ int forward_typed(const tcb200_topk_distill_t& p, const void* logits, const Entr
   attr[1].val.clusterDim.x = parts;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  TCB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, distill_forward_kernel<T>, static_cast<const T*>(logits), p.ld_logits, p.V, e,
+  cfg.numAttrs = parts > 1 ? 2 : 1;  // (a cluster of one is scheduled as slowly as any: 13 -> 22 us for 8192 x 600 f16)
+  const auto kernel = threads == 64 ? distill_forward_kernel<T, 64> : distill_forward_kernel<T, 256>;
+  TCB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(logits), p.ld_logits, p.V, e,
                                      p.temperature, loss, stats, parts));
   return TCB200_OK;
 }
@@ -411,7 +437,11 @@ int backward_typed(const tcb200_topk_distill_t& p, const void* logits, const Ent
   // (4096 x 131072 bf16, stretches of 8192 / 32768 / 65536 / 131072: 407 / 340 / 356 / 361 us)
   const int64_t fill = std::min<int64_t>(8ll * sms / p.N, p.V / 2048);
   const int parts = (int)std::max<int64_t>({1, fill, ceil_div(p.V, 32768)});
-  TCB200_CUDA_TRY(launch_pdl(distill_backward_kernel<T>, dim3((unsigned)(p.N * parts)), dim3(kThreads), (size_t)p.K * 8, s,
+  // at most 32 KB of entries and 8 KB of bits
+  const size_t smem = (size_t)p.K * 8 + (size_t)ceil_div(ceil_div(p.V, (int64_t)parts), (int64_t)64) * 16;
+  const int threads = threads_for(p, sms);
+  const auto kernel = threads == 64 ? distill_backward_kernel<T, 64> : distill_backward_kernel<T, 256>;
+  TCB200_CUDA_TRY(launch_pdl(kernel, dim3((unsigned)(p.N * parts)), dim3(threads), smem, s,
                              static_cast<const T*>(logits), p.ld_logits, p.V, e, p.temperature, stats, g, g_stride,
                              static_cast<T*>(dlogits), parts));
   return TCB200_OK;

@@ -372,6 +372,20 @@ def test_topk_distillation(cuda, dtype, n, v, k, ragged, temperature):
     check_kd(z, i, s, up, temperature, *step_kd(z, i, s, up, temperature))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v,k,ragged", [
+    (1200, 515, 5, True), (1300, 90, 120, False), (1184, 4099, 33, True), (1250, 8192, 128, False), (1250, 8193, 65, False), (2500, 31, 1, True),
+    (1300, 600, 129, True), (40, 500, 2000, False), (3, 70001, 4096, False)])
+def test_distillation_many_short_rows_and_equal_indices(cuda, dtype, n, v, k, ragged):
+    """Rows enough for small blocks, and (K > V, and every third entry a copy of the first) places that many entries share."""
+    z, i, s, up = make_kd(cuda, n, v, k, dtype, ragged, seed=n + v + k)
+    i[::2, ::3] = i[::2, :1]
+    got = step_kd(z, i, s, up, 2.0)
+    check_kd(z, i, s, up, 2.0, *got)
+    again = step_kd(z, i, s, up, 2.0)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
 def test_distillation_other_types_and_strides(cuda):
     n, v, k = 37, 5003, 24
     z, i, s, up = make_kd(cuda, n, v, k, torch.bfloat16, True, index=torch.int32, teacher_dtype=torch.float32)
