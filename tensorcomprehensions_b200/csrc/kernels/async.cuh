@@ -83,10 +83,16 @@ __device__ __forceinline__ uint32_t cluster_ctarank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-// all threads of all CTAs of the cluster
-__device__ __forceinline__ void cluster_sync_all() {
+// all threads of all CTAs of the cluster; the two halves for a CTA that has work of its own between them
+__device__ __forceinline__ void cluster_arrive() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  cluster_arrive();
+  cluster_wait();
 }
 // One arrival per warp on the barrier at the same shared-memory offset in CTA `rank` of the cluster.
 // Default semantics (release at CTA scope), as for a local arrival: the data the arrival publishes is

@@ -216,6 +216,8 @@ __global__ void __launch_bounds__(kThreads) distill_forward_kernel(const T* logi
   __shared__ float4 share[kThreads / 32];
   __shared__ float sums[kThreads / 32];
   __shared__ float2 gathered[kMaxCluster];
+  // A CTA's shared memory may be touched by its peers only once it runs: all say so here, and wait behind their stretch.
+  if (parts > 1) cluster_arrive();
   pdl_sync();
   const int rank = (int)(blockIdx.x % parts);
   const int64_t row = blockIdx.x / parts;
@@ -261,11 +263,14 @@ __global__ void __launch_bounds__(kThreads) distill_forward_kernel(const T* logi
     }
   block_join<kThreads>(r, t, scale, share);
   if (parts > 1) {
+    __syncwarp();
+    cluster_wait();
     if (threadIdx.x == 0) {
       uint32_t at;
       asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(smem_u32(&gathered[rank])));
       asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(r.top), "f"(r.sum) : "memory");
     }
+    __syncwarp();
     cluster_sync_all();
     if (rank != 0) return;
     r = Running();

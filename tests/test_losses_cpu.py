@@ -98,3 +98,20 @@ def test_cpp_entry_points(cuda):
     r = _run(_build("losses"))
     assert r.returncode == 0, r.stdout + r.stderr
     assert "losses ok (gpu=1)" in r.stdout
+
+
+def test_a_peers_shared_memory_is_touched_only_behind_a_cluster_barrier():
+    """In every kernel source: a store into another CTA's shared memory stands behind a wait of the same kernel on its cluster's barrier,
+    since a CTA that has not started has no shared memory to store into."""
+    import glob
+    import os
+    import re
+    kernels = os.path.join(os.path.dirname(cabi.__file__), "csrc", "kernels")
+    stores = 0
+    for path in glob.glob(os.path.join(kernels, "*.cu")) + glob.glob(os.path.join(kernels, "*.cuh")):
+        text = re.sub(r"//[^\n]*", "", open(path).read())
+        for body in re.split(r"\b__global__\b", text)[1:]:
+            for at in (m.start() for m in re.finditer(r"\bst\.(?:async\.)?shared::cluster", body)):
+                stores += 1
+                assert re.search(r"\bcluster_(?:wait|sync_all)\(\)", body[:at]), path
+    assert stores > 0

@@ -655,3 +655,16 @@ def test_refusals_on_the_device(cuda):
         tc.topk_distillation(z, i, s.clone().requires_grad_())
     with pytest.raises(RuntimeError):
         tc.topk_distillation(z, torch.zeros(4, 4097, device=cuda, dtype=torch.int64), torch.zeros(4, 4097, device=cuda))
+
+
+@pytest.mark.parametrize("v,parts", [(4096, 2), (8191, 2), (8192, 4), (16384, 8), (40000, 8)])
+def test_distillation_of_rows_split_over_clusters(cuda, v, parts):
+    """Clusters of every size with the shortest stretches they take, from a single one to more than the device holds at a time: CTAs of a
+    cluster that start apart leave the same bits."""
+    for n in (1, 3, 1183 // parts):
+        z, i, s, up = make_kd(cuda, n, v, 6, torch.float32, seed=v + n)
+        want = step_kd(z, i, s, up, 2.0)
+        check_kd(z, i, s, up, 2.0, *want)
+        for _ in range(20):
+            got = step_kd(z, i, s, up, 2.0)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
