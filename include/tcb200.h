@@ -278,8 +278,9 @@ int tcb200_linear_ce_backward(const tcb200_linear_ce_t* problem, const void* X, 
  *   dlogits(n,v) = T grad_loss[n] (p(v) - sum of q_k over the entries with indices[n,k] = v).
  * An index below 0, or a teacher logit of -inf, is no entry; a row without entries has loss 0 and gradient 0 whatever its
  * logits hold.  An index of V or more makes the row's loss and gradient NaN.  The same index twice counts twice.
- * stats[3n], stats[3n + 1]: maximum of the row's logits and sum of exp((logits - maximum) / T); stats[3n + 2]: log sum exp
- * of its entries' teacher logits / T (-inf: no entries, NaN: an index of V or more).  [N, 3], for the backward call. */
+ * stats[3n], stats[3n + 1]: maximum of the row's logits and sum of exp((logits - maximum) / T); stats[3n + 2]: log of the sum of
+ * exp((t - maximum of t) / T) over its entries' teacher logits t (-inf: no entries, NaN: an index of V or more).  [N, 3], for
+ * the backward call, which takes the maximum of t from the entries. */
 #define TCB200_TOPK_MAX 4096
 typedef struct tcb200_topk_distill {
   int64_t N, V, K;                     /* logits is [N, V], indices and teacher are [N, K], 1 <= K <= TCB200_TOPK_MAX */

@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(kThreads) distill_forward_kernel(const T* logi
     loss[row] = any_bad ? nan : none ? 0.f : temperature * temperature * sum;
     stats[3 * row] = r.top;
     stats[3 * row + 1] = r.sum;
-    stats[3 * row + 2] = any_bad ? nan : none ? -INFINITY : t.top * inv + log_weight;
+    stats[3 * row + 2] = any_bad ? nan : none ? -INFINITY : log_weight;
   }
 }
 
@@ -307,8 +307,11 @@ template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const T* logits, int64_t ld, int64_t v, Entries e,
                                                                     float temperature, const float* stats, const float* g,
                                                                     int64_t g_stride, T* dlogits, int parts) {
-  // q of the entries of this stretch, their places in it (-1: none), two bits a place: taken by an entry, by more than one
+  // Teacher logits, then q, of the entries of this stretch, their places in it (-1: none), two bits a place: taken by an entry,
+  // by more than one.  q comes from the difference to the largest teacher logit, as in the forward pass: exact where exp is not
+  // small, whatever the logits' size.  The maximum is found again here, among entries that are read anyway.
   extern __shared__ float entry_mem[];
+  __shared__ float tops[kThreads / 32];
   pdl_sync();
   const int64_t row = blockIdx.x / parts;
   int64_t first, last;
@@ -325,12 +328,16 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const T* log
   const bool none = log_weight == -INFINITY;
   float up = temperature * g[row * g_stride];
   if (log_weight != log_weight) up = log_weight;  // an index outside the vocabulary: the row is NaN
+  float best = -INFINITY;
   for (int j = threadIdx.x; j < e.k; j += kThreads) {
     const int64_t i = e.index(row, j);
-    const bool mine = i >= first && i < last && !none;
-    ei[j] = mine ? (int)(i - first) : -1;
-    eq[j] = mine ? exp2f((e.logit(row, j) * inv - log_weight) * kLog2e) : 0.f;
+    const float x = i >= 0 ? e.logit(row, j) : -INFINITY;
+    best = fmaxf(best, x);
+    ei[j] = i >= first && i < last && !none ? (int)(i - first) : -1;
+    eq[j] = x;
   }
+  for (int o = 16; o; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = best;
   constexpr int W = Vec<T>::n;
   const float weight = up / sum;
   auto grad = [&](float x) { return none ? 0.f : weight * exp_from(x, top, scale); };
@@ -366,8 +373,10 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const T* log
     out[at] = make1<T>(grad(load1(z + at)));
   }
   __syncthreads();  // the entries' places are written again behind this
+  for (int w = 0; w < kThreads / 32; ++w) best = fmaxf(best, tops[w]);
   for (int j = threadIdx.x; j < e.k; j += kThreads) {
     if (ei[j] < 0) continue;
+    eq[j] = exp2f(((eq[j] - best) * inv - log_weight) * kLog2e);
     const uint32_t bit = 1u << (ei[j] & 31);
     if (atomicOr(&taken[ei[j] >> 5], bit) & bit) atomicOr(&taken[words + (ei[j] >> 5)], bit);
   }

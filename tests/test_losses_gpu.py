@@ -668,3 +668,32 @@ def test_distillation_of_rows_split_over_clusters(cuda, v, parts):
         for _ in range(20):
             got = step_kd(z, i, s, up, 2.0)
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temperature", [0.5, 1.0, 3.0])
+@pytest.mark.parametrize("n,v,k", [(9, 4003, 9), (9, 20000, 700), (1300, 90, 40)])
+def test_distillation_teacher_rows_of_the_lowest_value_and_large_ones(cuda, dtype, temperature, n, v, k):
+    """The teacher's distribution follows from differences of its logits alone, in the loss and in the gradient: rows of the type's
+    lowest value are uniform, rows of large whole numbers are what the small differences between them say."""
+    z, i, s, up = make_kd(cuda, n, v, k, dtype, seed=n + k)
+    top = 60000 if dtype == torch.float16 else 2.0**20
+    s[0] = torch.finfo(dtype).min
+    s[1] = torch.finfo(dtype).min
+    s[1, 0] = 3
+    s[2] = (torch.randint(0, 8, (k,), generator=torch.Generator(device=cuda).manual_seed(1), device=cuda) + 16000).to(dtype)  # exact, but 16000 + 0 or 64 in bfloat16
+    s[3] = -s[2]
+    s[4] = top
+    s[5] = -top
+    s[6] = torch.finfo(dtype).max
+    s[7, ::2] = -math.inf
+    s[7, 1::2] = top
+    i[7, 1::3] = -1
+    rl, rz, p, q, _ = reference_kd(z, i, s, up, temperature)
+    loss, dz = step_kd(z, i, s, up, temperature)
+    # differences of the teacher's logits are at most 64 / T where their exp is not 0 on both sides, the student's (deviation 2.5) 30 / T
+    rel = 2.0**-20 * (4 + 94 / temperature)
+    assert ((loss.double() - rl).abs() <= temperature**2 * rel).all()
+    u = half_step(dtype)
+    tol = u * rz.abs() + (p + q) * rel + u * torch.finfo(dtype).tiny
+    assert ((dz.double() - rz).abs() <= tol).all(), "gradient off by %g of its tolerance" % ((dz.double() - rz).abs() / tol).max()
