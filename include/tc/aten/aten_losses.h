@@ -4,19 +4,31 @@
 //   auto g = tc::aten::linearCrossEntropyBackward(X, W, target, r[1], gradLoss);   // {dX, dW}
 //
 // The reference's operator library ends at the layers (tc/library); these follow its ATen entry points: checks that throw,
-// outputs on the device of the inputs, work on a caller's stream, no synchronisation.  Scratch memory comes from ATen's
-// allocator, call by call, so calls on different streams or in different captured graphs share none.
+// outputs on the device of the inputs, work on a caller's stream, no synchronisation.  The stream is ATen's current one of the
+// inputs' device, or the one that the call names, which is then ATen's current stream for the length of the call: copies,
+// kernels and the memory of outputs and scratch all follow its order.  Scratch memory comes from ATen's allocator, call by
+// call, so calls on different streams or in different captured graphs share none.  As with every ATen operator, inputs made on
+// another stream, and results read on one, need that stream's order (an event, recordStream).
 #pragma once
 
 #include <ATen/ATen.h>
 
 #include <cmath>
 #include <limits>
+#include <optional>
 #include <vector>
 
 #include "tc/core/check.h"
 #include "tc/core/cuda/cuda.h"
 #include "tcb200.h"
+
+// ATen's current stream through libtorch's C interface, which needs no CUDA headers (each returns 0 on success).
+struct CUDAStreamGuardOpaque;
+extern "C" {
+int32_t aoti_torch_get_current_cuda_stream(int32_t device, void** stream);
+int32_t aoti_torch_create_cuda_stream_guard(void* stream, int32_t device, CUDAStreamGuardOpaque** guard);
+int32_t aoti_torch_delete_cuda_stream_guard(CUDAStreamGuardOpaque* guard);
+}
 
 namespace tc {
 namespace aten {
@@ -56,6 +68,36 @@ inline int64_t lossGradStride(const at::Tensor& g, int64_t n, const at::Tensor& 
 }
 
 inline void lossStatus(int st, const char* what) { TC_CHECK(st == TCB200_OK) << what << ": " << tcb200_strerror(st); }
+
+// The stream of a call, ATen's current one while this lives.
+class LossStream {
+ public:
+  LossStream(const at::Tensor& like, const std::optional<tcb200_stream_t>& named) {
+    const int32_t device = static_cast<int32_t>(like.get_device());
+    void* current = nullptr;
+    TC_CHECK(aoti_torch_get_current_cuda_stream(device, &current) == 0) << "no current CUDA stream";
+    stream_ = static_cast<tcb200_stream_t>(current);
+    if (!named) return;
+    // handles that CUDA reserves for the default stream and for the calling thread's own
+    const auto legacy = reinterpret_cast<tcb200_stream_t>(1), perThread = reinterpret_cast<tcb200_stream_t>(2);
+    // ATen's allocator knows a stream by its handle, and this one is another stream in every thread
+    TC_CHECK(*named != perThread) << "cudaStreamPerThread is not supported: pass a stream of your own";
+    const tcb200_stream_t s = *named == legacy ? nullptr : *named;
+    if (s == stream_) return;
+    TC_CHECK(aoti_torch_create_cuda_stream_guard(s, device, &guard_) == 0) << "the stream cannot be made ATen's current one";
+    stream_ = s;
+  }
+  ~LossStream() {
+    if (guard_) aoti_torch_delete_cuda_stream_guard(guard_);
+  }
+  LossStream(const LossStream&) = delete;
+  LossStream& operator=(const LossStream&) = delete;
+  operator tcb200_stream_t() const { return stream_; }
+
+ private:
+  tcb200_stream_t stream_;
+  CUDAStreamGuardOpaque* guard_ = nullptr;
+};
 
 inline tcb200_linear_ce_t linearCe(const at::Tensor& X, const at::Tensor& W, const at::Tensor& target, int64_t ignoreIndex) {
   lossMatrix(X, "X", X);
@@ -107,9 +149,10 @@ inline tcb200_topk_distill_t topkDistill(const at::Tensor& logits, const at::Ten
 
 // Softmax cross entropy of z = X W^T against `target`, without keeping z: {loss [N], lse [N]}, float32.
 inline std::vector<at::Tensor> linearCrossEntropy(const at::Tensor& X, const at::Tensor& W, const at::Tensor& target,
-                                                  int64_t ignoreIndex = -100, tcb200_stream_t stream = nullptr) {
+                                                  int64_t ignoreIndex = -100, std::optional<tcb200_stream_t> stream = std::nullopt) {
   const tcb200_linear_ce_t p = detail::linearCe(X, W, target, ignoreIndex);
   WithCudaDevice dev((size_t)X.get_device());
+  const detail::LossStream on(X, stream);
   const at::Tensor t = target.contiguous();
   auto f32 = X.options().dtype(at::kFloat).requires_grad(false);
   at::Tensor loss = at::empty({p.N}, f32), lse = at::empty({p.N}, f32);
@@ -117,7 +160,7 @@ inline std::vector<at::Tensor> linearCrossEntropy(const at::Tensor& X, const at:
   detail::lossStatus(tcb200_linear_ce_workspace(&p, &bytes, nullptr), "linearCrossEntropy");
   at::Tensor ws = at::empty({bytes}, X.options().dtype(at::kByte).requires_grad(false));
   detail::lossStatus(tcb200_linear_ce_forward(&p, X.data_ptr(), W.data_ptr(), t.data_ptr(), loss.data_ptr<float>(),
-                                              lse.data_ptr<float>(), ws.data_ptr(), bytes, stream, nullptr),
+                                              lse.data_ptr<float>(), ws.data_ptr(), bytes, on, nullptr),
                      "linearCrossEntropy");
   return {loss, lse};
 }
@@ -126,12 +169,13 @@ inline std::vector<at::Tensor> linearCrossEntropy(const at::Tensor& X, const at:
 inline std::vector<at::Tensor> linearCrossEntropyBackward(const at::Tensor& X, const at::Tensor& W, const at::Tensor& target,
                                                           const at::Tensor& lse, const at::Tensor& gradLoss,
                                                           int64_t ignoreIndex = -100, bool needX = true, bool needW = true,
-                                                          tcb200_stream_t stream = nullptr) {
+                                                          std::optional<tcb200_stream_t> stream = std::nullopt) {
   const tcb200_linear_ce_t p = detail::linearCe(X, W, target, ignoreIndex);
   const int64_t stride = detail::lossGradStride(gradLoss, p.N, X);
   TC_CHECK(lse.is_cuda() && lse.get_device() == X.get_device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
            lse.numel() == p.N) << "lse must be the second result of linearCrossEntropy";
   WithCudaDevice dev((size_t)X.get_device());
+  const detail::LossStream on(X, stream);
   const at::Tensor t = target.contiguous();
   auto like = X.options().requires_grad(false);
   at::Tensor dX, dW;
@@ -142,20 +186,21 @@ inline std::vector<at::Tensor> linearCrossEntropyBackward(const at::Tensor& X, c
   at::Tensor ws = at::empty({bytes}, like.dtype(at::kByte));
   detail::lossStatus(tcb200_linear_ce_backward(&p, X.data_ptr(), W.data_ptr(), t.data_ptr(), lse.data_ptr<float>(),
                                                gradLoss.data_ptr<float>(), stride, needX ? dX.data_ptr() : nullptr,
-                                               needW ? dW.data_ptr() : nullptr, ws.data_ptr(), bytes, stream, nullptr),
+                                               needW ? dW.data_ptr() : nullptr, ws.data_ptr(), bytes, on, nullptr),
                      "linearCrossEntropyBackward");
   return {dX, dW};
 }
 
 // Distillation of `logits` [N, V] from a teacher's logits [N, K] at `indices`: {loss [N], stats [N, 3]}, float32.
 inline std::vector<at::Tensor> topkDistillation(const at::Tensor& logits, const at::Tensor& indices, const at::Tensor& teacher,
-                                                double temperature = 1.0, tcb200_stream_t stream = nullptr) {
+                                                double temperature = 1.0, std::optional<tcb200_stream_t> stream = std::nullopt) {
   const tcb200_topk_distill_t p = detail::topkDistill(logits, indices, teacher, temperature);
   WithCudaDevice dev((size_t)logits.get_device());
+  const detail::LossStream on(logits, stream);
   auto f32 = logits.options().dtype(at::kFloat).requires_grad(false);
   at::Tensor loss = at::empty({p.N}, f32), stats = at::empty({p.N, 3}, f32);
   detail::lossStatus(tcb200_topk_distill_forward(&p, logits.data_ptr(), indices.data_ptr(), teacher.data_ptr(),
-                                                 loss.data_ptr<float>(), stats.data_ptr<float>(), stream),
+                                                 loss.data_ptr<float>(), stats.data_ptr<float>(), on),
                      "topkDistillation");
   return {loss, stats};
 }
@@ -163,16 +208,17 @@ inline std::vector<at::Tensor> topkDistillation(const at::Tensor& logits, const 
 // Its gradient with respect to the logits.
 inline at::Tensor topkDistillationBackward(const at::Tensor& logits, const at::Tensor& indices, const at::Tensor& teacher,
                                            const at::Tensor& stats, const at::Tensor& gradLoss, double temperature = 1.0,
-                                           tcb200_stream_t stream = nullptr) {
+                                           std::optional<tcb200_stream_t> stream = std::nullopt) {
   const tcb200_topk_distill_t p = detail::topkDistill(logits, indices, teacher, temperature);
   const int64_t stride = detail::lossGradStride(gradLoss, p.N, logits);
   TC_CHECK(stats.is_cuda() && stats.get_device() == logits.get_device() && stats.scalar_type() == at::kFloat &&
            stats.is_contiguous() && stats.numel() == 3 * p.N) << "stats must be the second result of topkDistillation";
   WithCudaDevice dev((size_t)logits.get_device());
+  const detail::LossStream on(logits, stream);
   at::Tensor d = at::empty({p.N, p.V}, logits.options().requires_grad(false));
   detail::lossStatus(tcb200_topk_distill_backward(&p, logits.data_ptr(), indices.data_ptr(), teacher.data_ptr(),
                                                   stats.data_ptr<float>(), gradLoss.data_ptr<float>(), stride, d.data_ptr(),
-                                                  stream),
+                                                  on),
                      "topkDistillationBackward");
   return d;
 }

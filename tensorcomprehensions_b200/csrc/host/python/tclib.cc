@@ -1,7 +1,6 @@
 // pybind11 module over the ATen-facing C++ API (the reference's tensor_comprehensions/pybinds/tclib.cc).
 // Everything here goes through tc::aten::compile / run / profile / ATenAutotuner::tune; the extra
 // introspection helpers (sexpr, analyze, match) exist for the CPU-side tests.
-#include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
 #include <sstream>
@@ -93,14 +92,11 @@ struct OnDeviceOf {
 
 // ---- losses of a large-vocabulary head (tc/aten/aten_losses.h) as autograd functions ----
 // They run on the current stream of the tensors' device.
-tcb200_stream_t streamOf(const at::Tensor& t) {
-  return t.is_cuda() ? reinterpret_cast<tcb200_stream_t>(c10::cuda::getCurrentCUDAStream(t.get_device()).stream()) : nullptr;
-}
 
 struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& X, const at::Tensor& W,
                             const at::Tensor& target, int64_t ignoreIndex) {
-    auto r = tc::aten::linearCrossEntropy(X, W, target, ignoreIndex, streamOf(X));
+    auto r = tc::aten::linearCrossEntropy(X, W, target, ignoreIndex);
     ctx->saved_data["ignore_index"] = ignoreIndex;
     ctx->save_for_backward({X, W, target, r[1]});
     return r[0];
@@ -111,7 +107,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     const auto saved = ctx->get_saved_variables();
     auto r = tc::aten::linearCrossEntropyBackward(saved[0], saved[1], saved[2], saved[3], grads[0],
                                                   ctx->saved_data["ignore_index"].toInt(), ctx->needs_input_grad(0),
-                                                  ctx->needs_input_grad(1), streamOf(saved[0]));
+                                                  ctx->needs_input_grad(1));
     return {r[0], r[1], at::Tensor(), at::Tensor()};
   }
 };
@@ -119,7 +115,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
 struct TopkDistillation : torch::autograd::Function<TopkDistillation> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& indices,
                             const at::Tensor& teacher, double temperature) {
-    auto r = tc::aten::topkDistillation(logits, indices, teacher, temperature, streamOf(logits));
+    auto r = tc::aten::topkDistillation(logits, indices, teacher, temperature);
     ctx->saved_data["temperature"] = temperature;
     ctx->save_for_backward({logits, indices, teacher, r[1]});
     return r[0];
@@ -129,7 +125,7 @@ struct TopkDistillation : torch::autograd::Function<TopkDistillation> {
     if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
     const auto saved = ctx->get_saved_variables();
     return {tc::aten::topkDistillationBackward(saved[0], saved[1], saved[2], saved[3], grads[0],
-                                               ctx->saved_data["temperature"].toDouble(), streamOf(saved[0])),
+                                               ctx->saved_data["temperature"].toDouble()),
             at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
@@ -405,7 +401,7 @@ PYBIND11_MODULE(tclib, m) {
         [](const at::Tensor& X, const at::Tensor& W, const at::Tensor& target, int64_t ignoreIndex) {
           if (at::GradMode::is_enabled() && (X.requires_grad() || W.requires_grad()))
             return LinearCrossEntropy::apply(X, W, target, ignoreIndex);
-          return tc::aten::linearCrossEntropy(X, W, target, ignoreIndex, streamOf(X))[0];
+          return tc::aten::linearCrossEntropy(X, W, target, ignoreIndex)[0];
         });
   m.def("topk_distillation",
         [](const at::Tensor& logits, const at::Tensor& indices, const at::Tensor& teacher, double temperature) {
@@ -413,7 +409,7 @@ PYBIND11_MODULE(tclib, m) {
               << "topk_distillation gives the teacher no gradient: pass teacher.detach()";
           if (at::GradMode::is_enabled() && logits.requires_grad())
             return TopkDistillation::apply(logits, indices, teacher, temperature);
-          return tc::aten::topkDistillation(logits, indices, teacher, temperature, streamOf(logits))[0];
+          return tc::aten::topkDistillation(logits, indices, teacher, temperature)[0];
         });
 
   m.def("set_flag", [](const std::string& name, const std::string& value) {

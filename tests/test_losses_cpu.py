@@ -115,3 +115,39 @@ def test_a_peers_shared_memory_is_touched_only_behind_a_cluster_barrier():
                 stores += 1
                 assert re.search(r"\bcluster_(?:wait|sync_all)\(\)", body[:at]), path
     assert stores > 0
+
+
+def _build_with_streams():
+    """tests/cpp/losses_streams.cc, which makes streams with torch's C++ classes: those need the CUDA headers."""
+    import os
+    import subprocess
+    from torch.utils import cpp_extension
+    pkg = os.path.dirname(cabi.__file__)
+    src, exe = os.path.join(os.path.dirname(__file__), "cpp", "losses_streams.cc"), os.path.join(pkg, "build", "losses_streams")
+    os.makedirs(os.path.dirname(exe), exist_ok=True)
+    if not os.path.exists(exe) or any(os.path.getmtime(f) > os.path.getmtime(exe) for f in (src, os.path.join(pkg, "libtc_core.so"))):
+        tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
+        cmd = ["/usr/bin/g++", "-std=c++17", "-O1", "-w", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+               "-I" + os.path.join(os.path.dirname(pkg), "include"), "-I/usr/local/cuda/include"] + ["-I" + p for p in cpp_extension.include_paths()] + \
+              [src, "-o", exe, "-L" + pkg, "-ltc_core", "-ltcb200", "-L" + tlib, "-ltorch", "-ltorch_cpu", "-lc10", "-Wl,-rpath," + pkg,
+               "-Wl,-rpath," + tlib, "-Wl,--no-as-needed", "-ltorch_cuda", "-lc10_cuda", "-Wl,--as-needed", "-L/usr/local/cuda/lib64", "-lcudart"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        assert r.returncode == 0, r.stderr[-3000:]
+    return exe
+
+
+def test_cpp_entry_points_on_named_streams_build():
+    if torch.cuda.is_available():
+        pytest.skip("covered by the gpu variant")
+    from test_cpp_api import _run
+    r = _run(_build_with_streams())
+    assert r.returncode == 0, r.stdout + r.stderr
+    assert "losses on streams ok (gpu=0)" in r.stdout
+
+
+@pytest.mark.gpu
+def test_cpp_entry_points_on_named_streams(cuda):
+    from test_cpp_api import _run
+    r = _run(_build_with_streams())
+    assert r.returncode == 0, r.stdout + r.stderr
+    assert "losses on streams ok (gpu=1)" in r.stdout
