@@ -1,6 +1,7 @@
 // pybind11 module over the ATen-facing C++ API (the reference's tensor_comprehensions/pybinds/tclib.cc).
 // Everything here goes through tc::aten::compile / run / profile / ATenAutotuner::tune; the extra
 // introspection helpers (sexpr, analyze, match) exist for the CPU-side tests.
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <sstream>
@@ -93,6 +94,12 @@ struct OnDeviceOf {
 // ---- losses of a large-vocabulary head (tc/aten/aten_losses.h) as autograd functions ----
 // They run on the current stream of the tensors' device.
 
+// The losses have reverse-mode derivatives only: a tangent (torch.autograd.forward_ad) would be dropped without a word.
+void noTangent(std::initializer_list<at::Tensor> tensors, const char* what) {
+  for (const at::Tensor& t : tensors)
+    TC_CHECK(!torch::autograd::isFwGradDefined(t)) << what << " has no forward-mode derivative";
+}
+
 struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& X, const at::Tensor& W,
                             const at::Tensor& target, int64_t ignoreIndex) {
@@ -104,6 +111,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     TC_CHECK(!at::GradMode::is_enabled()) << "linear_cross_entropy has no second derivative";
     if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    noTangent({grads[0]}, "the gradient of linear_cross_entropy");
     const auto saved = ctx->get_saved_variables();
     auto r = tc::aten::linearCrossEntropyBackward(saved[0], saved[1], saved[2], saved[3], grads[0],
                                                   ctx->saved_data["ignore_index"].toInt(), ctx->needs_input_grad(0),
@@ -123,6 +131,7 @@ struct TopkDistillation : torch::autograd::Function<TopkDistillation> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     TC_CHECK(!at::GradMode::is_enabled()) << "topk_distillation has no second derivative";
     if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    noTangent({grads[0]}, "the gradient of topk_distillation");
     const auto saved = ctx->get_saved_variables();
     return {tc::aten::topkDistillationBackward(saved[0], saved[1], saved[2], saved[3], grads[0],
                                                ctx->saved_data["temperature"].toDouble()),
@@ -399,12 +408,14 @@ PYBIND11_MODULE(tclib, m) {
   // ---- losses of a large-vocabulary head: losses.py documents them ----
   m.def("linear_cross_entropy",
         [](const at::Tensor& X, const at::Tensor& W, const at::Tensor& target, int64_t ignoreIndex) {
+          noTangent({X, W}, "linear_cross_entropy");
           if (at::GradMode::is_enabled() && (X.requires_grad() || W.requires_grad()))
             return LinearCrossEntropy::apply(X, W, target, ignoreIndex);
           return tc::aten::linearCrossEntropy(X, W, target, ignoreIndex)[0];
         });
   m.def("topk_distillation",
         [](const at::Tensor& logits, const at::Tensor& indices, const at::Tensor& teacher, double temperature) {
+          noTangent({logits, teacher}, "topk_distillation");
           TC_CHECK(!(at::GradMode::is_enabled() && teacher.requires_grad()))
               << "topk_distillation gives the teacher no gradient: pass teacher.detach()";
           if (at::GradMode::is_enabled() && logits.requires_grad())

@@ -151,3 +151,20 @@ def test_cpp_entry_points_on_named_streams(cuda):
     r = _run(_build_with_streams())
     assert r.returncode == 0, r.stdout + r.stderr
     assert "losses on streams ok (gpu=1)" in r.stdout
+
+
+def test_tangents_are_refused():
+    """Forward-mode derivatives: a dual tensor does not require grad, and its tangent must not get lost."""
+    import torch.autograd.forward_ad as fwd
+    x, w, t = torch.zeros(4, 8), torch.zeros(16, 8), torch.zeros(4, dtype=torch.int64)
+    z, i, s = torch.zeros(4, 16), torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, 2)
+    with fwd.dual_level():
+        dual = lambda a: fwd.make_dual(a, torch.ones_like(a))  # noqa: E731
+        for args in ((dual(x), w, t), (x, dual(w), t)):
+            with pytest.raises(RuntimeError, match="linear_cross_entropy has no forward-mode derivative"):
+                tc.linear_cross_entropy(*args)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                tc.linear_cross_entropy(*args)
+        for args in ((dual(z), i, s), (z, i, dual(s))):
+            with pytest.raises(RuntimeError, match="topk_distillation has no forward-mode derivative"):
+                tc.topk_distillation(*args)

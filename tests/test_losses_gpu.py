@@ -697,3 +697,19 @@ def test_distillation_teacher_rows_of_the_lowest_value_and_large_ones(cuda, dtyp
     u = half_step(dtype)
     tol = u * rz.abs() + (p + q) * rel + u * torch.finfo(dtype).tiny
     assert ((dz.double() - rz).abs() <= tol).all(), "gradient off by %g of its tolerance" % ((dz.double() - rz).abs() / tol).max()
+
+
+def test_tangents_are_refused_on_the_device(cuda):
+    """Forward mode over a loss, and over its gradient."""
+    import torch.autograd.forward_ad as fwd
+    x, w, t, up = make_ce(cuda, 4, 8, 16, torch.float32)
+    z, i, s, uk = make_kd(cuda, 4, 16, 3, torch.float32)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda a: tc.linear_cross_entropy(a, w, t), (x,), (x,))
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda a: tc.topk_distillation(z, i, a), (s,), (s,))
+    x.requires_grad_(), z.requires_grad_()
+    with fwd.dual_level():
+        for loss, leaf, g in ((tc.linear_cross_entropy(x, w, t), x, up), (tc.topk_distillation(z, i, s), z, uk)):
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                torch.autograd.grad(loss, leaf, fwd.make_dual(g, g))
