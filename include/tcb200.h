@@ -242,8 +242,7 @@ int tcb200_assemble_shards(const void* gathered, void* out, int world, int64_t r
  * several streams, devices and captured graphs.  Everything is enqueued on `stream` of the current device; nothing
  * synchronises or allocates, and every call may be captured into a graph.  Sums and statistics are fp32, each output is
  * rounded to its type once, and results do not depend on timing (no atomics on values).
- * A kernel whose bounded wait gives up makes the outputs NaN (dW: its first element) and stores a code in *dev_status
- * (optional). */
+ * A kernel whose bounded wait gives up makes all of the call's outputs NaN and stores a code in *dev_status (optional). */
 enum { TCB200_F32 = 0, TCB200_F16 = 1, TCB200_BF16 = 2 };
 
 /* Softmax cross entropy of the linear layer z = X W^T, without keeping z:

@@ -168,3 +168,31 @@ def test_tangents_are_refused():
         for args in ((dual(z), i, s), (z, i, dual(s))):
             with pytest.raises(RuntimeError, match="topk_distillation has no forward-mode derivative"):
                 tc.topk_distillation(*args)
+
+
+def _build_gave_up():
+    import os
+    import subprocess
+    from tensorcomprehensions_b200 import _build
+    kernels, exe = os.path.join(_build.CSRC, "kernels"), os.path.join(_build.PKG, "build", "losses_gave_up")
+    src = os.path.join(os.path.dirname(__file__), "cpp", "losses_gave_up.cu")
+    os.makedirs(os.path.dirname(exe), exist_ok=True)
+    if not os.path.exists(exe) or any(os.path.getmtime(f) > os.path.getmtime(exe) for f in (src, os.path.join(_build.PKG, "libtcb200.so"))):
+        r = subprocess.run([_build._nvcc()] + _build.NVCC_FLAGS + ["-I" + _build.INCLUDE, "-I" + kernels, src, "-o", exe], capture_output=True, text=True)
+        assert r.returncode == 0, r.stderr[-3000:]
+    return exe
+
+
+def test_gradients_behind_a_wait_that_gave_up_build():
+    if torch.cuda.is_available():
+        pytest.skip("covered by the gpu variant")
+    from test_cpp_api import _run
+    r = _run(_build_gave_up())
+    assert r.returncode == 0 and "gave up ok (gpu=0)" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.gpu
+def test_gradients_behind_a_wait_that_gave_up(cuda):
+    from test_cpp_api import _run
+    r = _run(_build_gave_up())
+    assert r.returncode == 0 and "gave up ok (gpu=1)" in r.stdout, r.stdout + r.stderr
