@@ -131,6 +131,7 @@ inline tcb200_topk_distill_t topkDistill(const at::Tensor& logits, const at::Ten
   TC_CHECK(indices.size(1) >= 1 && indices.size(1) <= TCB200_TOPK_MAX) << "a row must have 1 to " << TCB200_TOPK_MAX << " entries";
   const float t = static_cast<float>(temperature);
   TC_CHECK(t > 0.f && std::isfinite(t)) << "the temperature must be positive and finite";
+  TC_CHECK(std::isnormal(t * t)) << "the temperature's square must be a normal float32 number";
   tcb200_topk_distill_t p = {};
   p.N = logits.size(0);
   p.V = logits.size(1);

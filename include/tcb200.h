@@ -284,7 +284,7 @@ int tcb200_linear_ce_backward(const tcb200_linear_ce_t* problem, const void* X, 
 typedef struct tcb200_topk_distill {
   int64_t N, V, K;                     /* logits is [N, V], indices and teacher are [N, K], 1 <= K <= TCB200_TOPK_MAX */
   int64_t ld_logits, ld_indices, ld_teacher; /* elements between rows; dlogits is dense */
-  float temperature;                   /* > 0, finite */
+  float temperature;                   /* T > 0 whose square is a normal float (2^-63 <= T < 2^64) */
   int32_t logits_dtype, teacher_dtype; /* TCB200_F32 / F16 / BF16 */
   int32_t index_bytes;                 /* 4 or 8 */
 } tcb200_topk_distill_t;

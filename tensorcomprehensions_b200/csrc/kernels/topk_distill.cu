@@ -393,12 +393,19 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const T* log
   }
 }
 
+// The loss carries T^2 and the exponents log2(e) / T: T^2 has to be a normal number, or the loss is infinite, NaN or lost (then 1 / T
+// is one too: T lies between 2^-63 and 2^64).
+bool temperature_ok(float t) {
+  const float square = t * t;
+  return t > 0.f && square >= 1.17549435e-38f && square <= 3.402823466e38f;
+}
+
 int check(const tcb200_topk_distill_t* p) {
   if (!p) return TCB200_ERR_INVALID_ARGUMENT;
   auto type_ok = [](int t) { return t == TCB200_F32 || t == TCB200_F16 || t == TCB200_BF16; };
   if (p->N < 0 || p->V < 1 || p->K < 1 || p->ld_logits < p->V || p->ld_indices < p->K || p->ld_teacher < p->K ||
       !type_ok(p->logits_dtype) || !type_ok(p->teacher_dtype) || (p->index_bytes != 4 && p->index_bytes != 8) ||
-      !(p->temperature > 0.f) || !(p->temperature <= 3.402823466e38f))
+      !temperature_ok(p->temperature))
     return TCB200_ERR_INVALID_ARGUMENT;
   if (p->K > TCB200_TOPK_MAX || p->V >= (1ll << 31) || p->N >= (1ll << 27)) return TCB200_ERR_TOO_LARGE;
   return TCB200_OK;

@@ -33,7 +33,7 @@ def topk_distillation(logits, indices, teacher, temperature=1.0):
         loss[n] = T^2 sum_k q[k] (ln q[k] - ln p[indices[n, k]])
 
     logits [N, V] and teacher [N, K]: float32, float16 or bfloat16; indices [N, K]: int32 or int64; all dense along their
-    last dimension; 1 <= K <= 4096.  An index below 0, or a teacher logit of -inf, is no entry; a row without entries has
+    last dimension; 1 <= K <= 4096; T > 0, its square a normal float32 number (2^-63 <= T < 2^64).  An index below 0, or a teacher logit of -inf, is no entry; a row without entries has
     loss 0 and gradient 0; an index of V or more makes the row's loss and gradient NaN; an index that stands twice counts
     twice.  The gradient is that of the logits, in their type; the teacher gets none.  A wrong type, size, stride,
     device or temperature raises RuntimeError."""

@@ -196,3 +196,14 @@ def test_gradients_behind_a_wait_that_gave_up(cuda):
     from test_cpp_api import _run
     r = _run(_build_gave_up())
     assert r.returncode == 0 and "gave up ok (gpu=1)" in r.stdout, r.stdout + r.stderr
+
+
+def test_temperatures_whose_square_is_no_normal_number_are_refused():
+    """At 1e-39, 1 / T is infinite and the loss NaN; at 1e-20, T^2 is lost; at 1e20 it is infinite."""
+    L = cabi.lib()
+    for temperature in (1e-45, 1e-39, 1e-38, 1e-20, 1.0e-19, 2.0**64, 1e20, 3e38):
+        r = ctypes.byref(kd(N=0, temperature=temperature))   # N = 0 would succeed if the check let it through
+        assert L.tcb200_topk_distill_forward(r, PTR, PTR, PTR, PTR, PTR, None) == -1, temperature
+        assert L.tcb200_topk_distill_backward(r, PTR, PTR, PTR, PTR, PTR, 1, PTR, None) == -1, temperature
+    for temperature in (2.0**-63, 1e-3, 1.0, 100.0, 1e19):
+        assert L.tcb200_topk_distill_forward(ctypes.byref(kd(N=0, temperature=temperature)), PTR, PTR, PTR, PTR, PTR, None) == 0, temperature

@@ -713,3 +713,22 @@ def test_tangents_are_refused_on_the_device(cuda):
         for loss, leaf, g in ((tc.linear_cross_entropy(x, w, t), x, up), (tc.topk_distillation(z, i, s), z, uk)):
             with pytest.raises(RuntimeError, match="no forward-mode derivative"):
                 torch.autograd.grad(loss, leaf, fwd.make_dual(g, g))
+
+
+def test_distillation_extreme_temperatures(cuda):
+    z, i, s, up = make_kd(cuda, 4, 300, 3, torch.float32)
+    for temperature in (1e-39, 1e-20, 1e20):
+        with pytest.raises(RuntimeError, match="square must be a normal float32 number"):
+            tc.topk_distillation(z, i, s, temperature)
+    # the coldest one accepted: each side puts all of itself on its largest logit
+    z[:, 0], z[:, 1] = 20, 20.5
+    i[:, 0], i[:, 1], i[:, 2] = 1, 5, 6
+    s[:, 0], s[:, 1], s[:, 2] = 4, 3, 2
+    loss, dz = step_kd(z, i, s, up, 2.0**-63)
+    assert (loss == 0).all() and (dz == 0).all()
+    # the hottest: both are uniform over their places, p is 1 / 300 and q 1 / 3
+    _, dz = step_kd(z, i, s, up, 1e19)
+    want = torch.full((4, 300), 1 / 300, device=cuda, dtype=torch.float64)
+    want[:, [1, 5, 6]] -= 1 / 3
+    want *= 1e19 * up.double()[:, None]
+    assert ((dz.double() - want).abs() <= 2.0**-18 * want.abs()).all()
