@@ -732,3 +732,20 @@ def test_distillation_extreme_temperatures(cuda):
     want[:, [1, 5, 6]] -= 1 / 3
     want *= 1e19 * up.double()[:, None]
     assert ((dz.double() - want).abs() <= 2.0**-18 * want.abs()).all()
+
+
+@pytest.mark.parametrize("temperature", [1.0, 2.0])
+@pytest.mark.parametrize("n,v", [(5, 2003), (1300, 515)])
+def test_distillation_small_probabilities_keep_float32_accuracy(cuda, temperature, n, v):
+    """Differences of logits are exact here and the row's sum is its largest element's 1 and almost nothing else, so that a probability far
+    from the maximum is off by expf's two units (2^-22) and three roundings (2^-24 each) alone, however far it is."""
+    g = torch.Generator(device=cuda).manual_seed(2)
+    z = -torch.randint(20 * 64, 80 * 64, (n, v), generator=g, device=cuda).float() / 64 * temperature
+    z[:, 7] = 0
+    i = torch.tensor([7, 9, 11], device=cuda).expand(n, 3).contiguous()
+    s = torch.randn(n, 3, generator=g, device=cuda)
+    up = torch.rand(n, generator=g, device=cuda) + 0.5
+    _, want, _, _, _ = reference_kd(z, i, s, up, temperature)
+    _, dz = step_kd(z, i, s, up, temperature)
+    rest = [k for k in range(v) if k not in (7, 9, 11)]
+    assert ((dz.double() - want).abs()[:, rest] <= 2.0**-21 * want.abs()[:, rest]).all()
