@@ -260,19 +260,24 @@ struct Splits {
   int kb, products, pairs;
 };
 constexpr int kRowThreads = 512;
+// float16 keeps dZ / max|g| with 2^14 (GradEpi): a row's small probabilities leave its range as |g| / max|g| falls, which costs dX of
+// the row 1e-3 of itself at 2^-24, 3e-2 at 2^-32 and all from 2^-39 on.  From this share down (where nothing is lost yet) a row's
+// dZ has a power of two of its own for dX.  dW, a sum over rows, takes the common scale: what it loses, 2^-39 max|g|, is below
+// float16's steps unless max|g| passes 2^15.
+constexpr float kSmallShare = 1.f / 65536;
 template <typename T, typename Index>
 __global__ void __launch_bounds__(kRowThreads, 2) rows_kernel(const Index* target, int64_t n, int64_t v, int64_t ignore,
                                                            const float* g, int64_t g_stride, const float* lse, Rows r,
                                                            const T* x, int64_t ld, int64_t d, int64_t dp, Planes o, Splits sp) {
   __shared__ int before_of[kRowThreads / 32], all_of[kRowThreads / 32];
-  __shared__ float top_of[kRowThreads / 32];
+  __shared__ float top_of[kRowThreads / 32], least_of[kRowThreads / 32];
   __shared__ int list[kRowThreads];
   pdl_sync();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t per_block = (n + gridDim.x - 1) / gridDim.x;
   const int64_t r0 = min(n, blockIdx.x * per_block), r1 = min(n, r0 + per_block);
   int before = 0, all = 0;
-  float top = 0.f;
+  float top = 0.f, least = INFINITY;
 #pragma unroll 4
   for (int64_t i = threadIdx.x; i < n; i += kRowThreads) {
     const bool live = (int64_t)target[i] != ignore;
@@ -281,17 +286,20 @@ __global__ void __launch_bounds__(kRowThreads, 2) rows_kernel(const Index* targe
     if (g && live) {
       const float ax = fabsf(g[i * g_stride]);
       if (ax <= 3.402823466e38f) top = fmaxf(top, ax);  // the largest finite one: not NaN, not infinite
+      if (ax > 0.f) least = fminf(least, ax);
     }
   }
   for (int o = 16; o; o >>= 1) {
     before += __shfl_xor_sync(0xffffffffu, before, o);
     all += __shfl_xor_sync(0xffffffffu, all, o);
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
   }
   if (lane == 0) {
     before_of[warp] = before;
     all_of[warp] = all;
     top_of[warp] = top;
+    least_of[warp] = least;
   }
   __syncthreads();
   before = all = 0;
@@ -299,11 +307,14 @@ __global__ void __launch_bounds__(kRowThreads, 2) rows_kernel(const Index* targe
     before += before_of[w];
     all += all_of[w];
     top = fmaxf(top, top_of[w]);
+    least = fminf(least, least_of[w]);
   }
+  const float small = top * kSmallShare;  // rows of a smaller |g| have a scale of their own in dX
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     r.head->live = all;
     r.head->status = 0;
     r.head->gscale = top > 0.f ? top : 1.f;
+    r.head->spread = r.share_x && least < small ? all : 0;
     const int64_t tiles_m = (all + (int64_t)kTile - 1) / kTile, tiles = tiles_m * sp.tiles_n;
     r.head->splits = tiles == 0 || tiles > 1 << 20
                          ? 1
@@ -333,7 +344,15 @@ __global__ void __launch_bounds__(kRowThreads, 2) rows_kernel(const Index* targe
         // dZ is kept with g / max|g|: where all rows share one g, as under a mean, that is exactly 1 and the rounding
         // of dZ to 16 bits does not meet g's significand
         const float x = g[i * g_stride];
-        r.share[before + at] = !inside ? __int_as_float(0x7fffffff) : top > 0.f ? x / top : x;
+        const float share = !inside ? __int_as_float(0x7fffffff) : top > 0.f ? x / top : x;
+        r.share[before + at] = share;
+        if (r.share_x) {
+          const bool own = inside && x != 0.f && fabsf(x) < small;
+          int e = 0;
+          const float part = own ? frexpf(x, &e) : share;
+          r.share_x[before + at] = part;
+          r.factor_x[before + at] = own ? ldexpf(1.f, e) : top > 0.f ? top : 1.f;
+        }
         r.lse[before + at] = lse[i];
       }
     }
@@ -628,7 +647,7 @@ struct Layout {
   bool few_fwd, few_bwd;         // the kernels for few rows: nothing is packed, no dZ is kept
   int64_t fwd_bytes, bwd_bytes;
   // byte offsets
-  int64_t place, target, share, lse, hit, part, x, x_scaled, x_factor, w_fwd, w_fwd_factor, w_bwd, w_bwd_scaled, w_bwd_factor, dz,
+  int64_t place, target, share, lse, share_x, factor_x, hit, part, x, x_scaled, x_factor, w_fwd, w_fwd_factor, w_bwd, w_bwd_scaled, w_bwd_factor, dz,
       sums;
 };
 
@@ -681,6 +700,8 @@ int layout_of(const tcb200_linear_ce_t* q, int sms, Layout* l) {
   l->target = take(l->n_pad * 4);
   l->share = take(l->n_pad * 4);
   l->lse = take(l->n_pad * 4);
+  l->share_x = take(p.dtype == TCB200_F16 ? l->n_pad * 4 : 0);
+  l->factor_x = take(p.dtype == TCB200_F16 ? l->n_pad * 4 : 0);
   // X: the plain planes, unless float32 goes forward, and the scaled ones of float32
   const int64_t x_plane = l->few_fwd && l->few_bwd ? 0 : l->n_pad * l->dp * 2;
   l->x_factor = take(f32 ? l->n_pad * 4 : 0);
@@ -714,6 +735,7 @@ Rows rows_of(char* ws, const Layout& l) {
   r.target = reinterpret_cast<int*>(ws + l.target);
   r.share = reinterpret_cast<float*>(ws + l.share);
   r.lse = reinterpret_cast<float*>(ws + l.lse);
+  r.share_x = r.factor_x = nullptr;
   return r;
 }
 
@@ -801,13 +823,14 @@ int backward_typed(const tcb200_linear_ce_t& p, const Layout& l, const void* W, 
                       reinterpret_cast<float*>(ws + l.w_bwd_factor), l.bwd_piece * l.dp};
   float* sums = reinterpret_cast<float*>(ws + l.sums);
   const int* live = &r.head->live;
+  const float* share = dX && r.share_x ? r.share_x : r.share;
   int st;
   for (int64_t v0 = 0; v0 < p.V; v0 += l.bwd_piece) {
     const int64_t v = std::min(l.bwd_piece, p.V - v0), ld = l.bwd_piece;
     pg::Operand zw, w;
     if ((st = w_operands(p, l, W, v0, v, packed, sms, s, &zw, &w)) != TCB200_OK) return st;
     uint16_t* dz = reinterpret_cast<uint16_t*>(ws + l.dz);
-    const GradEpi<TYPE> ge{r.head, r.target, r.share, r.lse, ld, v0, v, reinterpret_cast<const float*>(ws + l.x_factor), packed.factor};
+    GradEpi<TYPE> ge{r.head, r.target, share, r.lse, ld, v0, v, reinterpret_cast<const float*>(ws + l.x_factor), packed.factor};
     CUtensorMap tc;
     if ((st = pg::make_out_map(&tc, {dz, ld, l.n_pad, ld, l.planes, l.n_pad * ld}, 2)) != TCB200_OK) return st;
     st = pg::launch_columns<false, false>(l.bwd_bn, zx, zw, TYPE == kBF16, gemm_args(p.N, v, p.D, live, 0, status, f32 ? 3 : 1, false), tc,
@@ -821,6 +844,13 @@ int backward_typed(const tcb200_linear_ce_t& p, const Layout& l, const void* W, 
       pg::Args a = gemm_args(p.N, p.D, v, live, 0, status, products, false);
       a.splits = &r.head->splits;
       if ((st = pg::launch<256, false, true>(z, w, bf16, a, tc, se, device, sms, s)) != TCB200_OK) return st;
+    }
+    if (dW && share != r.share) {  // dZ once more with the common scale, where some row had another: no tile otherwise
+      ge.share = r.share;
+      if ((st = pg::make_out_map(&tc, {dz, ld, l.n_pad, ld, l.planes, l.n_pad * ld}, 2)) != TCB200_OK) return st;
+      st = pg::launch_columns<false, false>(l.bwd_bn, zx, zw, false, gemm_args(p.N, v, p.D, &r.head->spread, 0, status, 1, false), tc, ge,
+                                            device, sms, s);
+      if (st != TCB200_OK) return st;
     }
     if (dW) {
       T* out = dW + v0 * p.D;
@@ -920,8 +950,12 @@ int tcb200_linear_ce_backward(const tcb200_linear_ce_t* problem, const void* X, 
   if ((st = current_device(&device)) != TCB200_OK) return st;
   const int sms = sm_count(device);
   char* ws = static_cast<char*>(workspace);
-  const Rows r = rows_of(ws, l);
+  Rows r = rows_of(ws, l);
   int* status = &r.head->status;
+  if (p.dtype == TCB200_F16 && dX && !l.few_bwd) {
+    r.share_x = reinterpret_cast<float*>(ws + l.share_x);
+    r.factor_x = reinterpret_cast<float*>(ws + l.factor_x);
+  }
   if (l.few_bwd)
     return few_backward(p, X, W, target, lse, grad_loss, grad_stride, r, reinterpret_cast<float*>(ws + l.sums),
                         l.sum_rows * l.dp, l.dp, dX, dW, device, sms, s);

@@ -16,6 +16,7 @@ struct Head {
   int status;    // a bounded wait that gave up
   float gscale;  // largest |g| of the live rows
   int splits;    // partial sums of dX
+  int spread;    // live rows where some row of dX has a scale of its own, else 0 (float16)
 };
 
 struct Rows {
@@ -23,6 +24,8 @@ struct Rows {
   int* place;     // [n] row -> live row, -1 without a target
   int* target;    // [n_pad] of a live row; -1: outside [0, V)
   float* share;   // [n_pad] g of a live row / gscale (backward)
+  float* share_x; // [n_pad] null, or g / factor_x: what dZ is formed with for dX (float16)
+  float* factor_x;// [n_pad] null, or gscale, or the power of two that is a row's own scale
   float* lse;     // [n_pad] of a live row (backward)
 };
 

@@ -20,13 +20,14 @@ __global__ void __launch_bounds__(256) finish_kernel(Rows r, const float* sums, 
   if (bad && dw)
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < dw_elems; i += (int64_t)gridDim.x * blockDim.x) dw[i] = from_float<T>(nan);
   if (!dx) return;
-  const float k = r.head->gscale * scale;
+  const float gscale = r.head->gscale;
   const int splits = r.head->splits;
   const int64_t plane = ((int64_t)r.head->live + pg::kTile - 1) / pg::kTile * pg::kTile * ld;
   const int64_t per_row = ld / 8;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n * per_row; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t row = i / per_row, c = (i % per_row) * 8;
     const int at = r.place[row];
+    const float k = (at >= 0 && r.factor_x ? r.factor_x[at] : gscale) * scale;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (at >= 0) {
 #pragma unroll 4

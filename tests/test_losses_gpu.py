@@ -749,3 +749,36 @@ def test_distillation_small_probabilities_keep_float32_accuracy(cuda, temperatur
     _, dz = step_kd(z, i, s, up, temperature)
     rest = [k for k in range(v) if k not in (7, 9, 11)]
     assert ((dz.double() - want).abs()[:, rest] <= 2.0**-21 * want.abs()[:, rest]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,d,v", [(60, 64, 3000), (300, 72, 1003)])
+def test_gradient_scales_far_from_each_other(cuda, dtype, n, d, v):
+    """Rows whose gradients lie far apart, as of weights under a loss scale: each row of dX as near as any other."""
+    x, w, t, _ = make_ce(cuda, n, d, v, dtype, 0.1)
+    for top, bottom in ((17, -24), (10, -2), (0, -16), (-10, -40)):
+        up = torch.exp2(torch.linspace(top, bottom, n, device=cuda)) * torch.where(torch.arange(n, device=cuda) % 3 == 0, -1.3, 1.0)
+        up[n // 2] = 0
+        loss, dx, dw = step_ce(x, w, t, up)
+        # the bounds of check_ce with p itself, which holds for gradients of either sign; what lies above a type's largest value
+        # (65504, under the scales of 2^17) is infinite in it
+        _, rx, rw, dz, delta = reference_ce(x, w, t, up)
+        u, most, tiny = half_step(dtype), torch.finfo(dtype).max, torch.finfo(dtype).tiny
+        live = (t != -100)[:, None]
+        p = torch.softmax((x.double() * live) @ w.double().t(), 1) * up.double().abs()[:, None] * live * (2 * delta + 2.0**-18)[:, None]
+        for got, ref, err in ((dx, rx, (dz.abs() * (u + (128 + v / 256) * 2.0**-23) + p) @ w.double().abs()),
+                              (dw, rw, (dz.abs() * (u + (128 + n / 256) * 2.0**-23) + p).t() @ (x.double() * live).abs())):
+            err = err + u * ref.abs() + u * tiny
+            over = ref.abs() + err > most
+            assert ((got.double() - ref).abs() <= err)[~over].all(), "off by %g of its tolerance" % ((got.double() - ref).abs() / err)[~over].max()
+            assert ((got.double() * ref.sign())[over] >= (ref.abs() - err).clamp(max=most)[over]).all()
+        xs = x.detach().requires_grad_()
+        (only,) = torch.autograd.grad(tc.linear_cross_entropy(xs, w, t), xs, up)
+        assert torch.equal(only, dx)
+        ws = w.detach().requires_grad_()
+        (only,) = torch.autograd.grad(tc.linear_cross_entropy(x, ws, t), ws, up)
+        assert torch.equal(only, dw)
+        # a row's own scale changes nothing for the others
+        big = up.abs() >= up.abs().max() * 2.0**-16
+        alone = torch.where(big, up, torch.zeros_like(up))
+        assert torch.equal(step_ce(x, w, t, alone)[1][big], dx[big])
