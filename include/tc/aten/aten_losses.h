@@ -172,12 +172,12 @@ inline std::vector<at::Tensor> linearCrossEntropyBackward(const at::Tensor& X, c
                                                           int64_t ignoreIndex = -100, bool needX = true, bool needW = true,
                                                           std::optional<tcb200_stream_t> stream = std::nullopt) {
   const tcb200_linear_ce_t p = detail::linearCe(X, W, target, ignoreIndex);
-  const int64_t stride = detail::lossGradStride(gradLoss, p.N, X);
   TC_CHECK(lse.is_cuda() && lse.get_device() == X.get_device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
            lse.numel() == p.N) << "lse must be the second result of linearCrossEntropy";
   WithCudaDevice dev((size_t)X.get_device());
   const detail::LossStream on(X, stream);
-  const at::Tensor t = target.contiguous();
+  const at::Tensor t = target.contiguous(), g = gradLoss.resolve_neg();  // (a view that stands for its negative is copied)
+  const int64_t stride = detail::lossGradStride(g, p.N, X);
   auto like = X.options().requires_grad(false);
   at::Tensor dX, dW;
   if (needX) dX = at::empty({p.N, p.D}, like);
@@ -186,7 +186,7 @@ inline std::vector<at::Tensor> linearCrossEntropyBackward(const at::Tensor& X, c
   detail::lossStatus(tcb200_linear_ce_workspace(&p, nullptr, &bytes), "linearCrossEntropyBackward");
   at::Tensor ws = at::empty({bytes}, like.dtype(at::kByte));
   detail::lossStatus(tcb200_linear_ce_backward(&p, X.data_ptr(), W.data_ptr(), t.data_ptr(), lse.data_ptr<float>(),
-                                               gradLoss.data_ptr<float>(), stride, needX ? dX.data_ptr() : nullptr,
+                                               g.data_ptr<float>(), stride, needX ? dX.data_ptr() : nullptr,
                                                needW ? dW.data_ptr() : nullptr, ws.data_ptr(), bytes, on, nullptr),
                      "linearCrossEntropyBackward");
   return {dX, dW};
@@ -211,14 +211,15 @@ inline at::Tensor topkDistillationBackward(const at::Tensor& logits, const at::T
                                            const at::Tensor& stats, const at::Tensor& gradLoss, double temperature = 1.0,
                                            std::optional<tcb200_stream_t> stream = std::nullopt) {
   const tcb200_topk_distill_t p = detail::topkDistill(logits, indices, teacher, temperature);
-  const int64_t stride = detail::lossGradStride(gradLoss, p.N, logits);
   TC_CHECK(stats.is_cuda() && stats.get_device() == logits.get_device() && stats.scalar_type() == at::kFloat &&
            stats.is_contiguous() && stats.numel() == 3 * p.N) << "stats must be the second result of topkDistillation";
   WithCudaDevice dev((size_t)logits.get_device());
   const detail::LossStream on(logits, stream);
+  const at::Tensor g = gradLoss.resolve_neg();
+  const int64_t stride = detail::lossGradStride(g, p.N, logits);
   at::Tensor d = at::empty({p.N, p.V}, logits.options().requires_grad(false));
   detail::lossStatus(tcb200_topk_distill_backward(&p, logits.data_ptr(), indices.data_ptr(), teacher.data_ptr(),
-                                                  stats.data_ptr<float>(), gradLoss.data_ptr<float>(), stride, d.data_ptr(),
+                                                  stats.data_ptr<float>(), g.data_ptr<float>(), stride, d.data_ptr(),
                                                   on),
                      "topkDistillationBackward");
   return d;

@@ -782,3 +782,19 @@ def test_gradient_scales_far_from_each_other(cuda, dtype, n, d, v):
         big = up.abs() >= up.abs().max() * 2.0**-16
         alone = torch.where(big, up, torch.zeros_like(up))
         assert torch.equal(step_ce(x, w, t, alone)[1][big], dx[big])
+
+
+def test_a_gradient_that_is_a_negated_view(cuda):
+    """Behind complex arithmetic autograd hands on views that stand for the negative of what memory holds."""
+    x, w, t, up = make_ce(cuda, 40, 64, 300, torch.float32)
+    z, i, s, uk = make_kd(cuda, 40, 300, 5, torch.float32)
+    for want, leaf, loss, g in ((step_ce(x, w, t, up)[1], x, lambda a: tc.linear_cross_entropy(a, w, t), up),
+                                (step_kd(z, i, s, uk)[1], z, lambda a: tc.topk_distillation(a, i, s), uk)):
+        leaf = leaf.detach().requires_grad_()
+        view = torch.imag(torch.complex(g, -g).conj())
+        assert view.is_neg() and torch.equal(view, g)
+        (got,) = torch.autograd.grad(loss(leaf), leaf, view)
+        assert torch.equal(got, want)
+        # the imaginary part's gradient of a conjugate: -g
+        (got,) = torch.autograd.grad(torch.complex(torch.zeros_like(g), loss(leaf)).conj(), leaf, torch.complex(g, g))
+        assert torch.equal(got, -want)
