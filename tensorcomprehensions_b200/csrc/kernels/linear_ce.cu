@@ -98,10 +98,10 @@ using pg::kTile;
 __device__ __forceinline__ uint16_t bits(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
 __device__ __forceinline__ uint16_t bits(__half v) { return __half_as_ushort(v); }
 
-// float32 operands.  The logits take two f16 planes of the row scaled by a power of two, v 2^e = h0 + h1: the row's largest
-// value lies in [2^14, 2^15), values down to 2^-17 of it keep 22 significand bits and smaller ones 2^-40 of it.  Three
-// products h1 h0 + h0 h1 + h0 h0 then give z to fp32's accuracy, half of what bf16 planes need, and 2^-e is taken off in the
-// epilogue.  The gradient's products sum over the rows that such scales belong to, so they take three bf16 planes without
+// float32 operands.  The logits take two f16 planes of the row scaled by a power of two, v 2^e = h0 + 2^-11 h1: the row's largest
+// value lies in [2^14, 2^15), values down to 2^-29 of it keep 22 significand bits and smaller ones 2^-50 of it (with h1 unscaled:
+// 2^-17 and 2^-40, and a row with a value 2^24 times the others had its logits off by 2^-16).  Three products, 2^-11 (h1 h0 + h0 h1)
+// + h0 h0, then give z to fp32's accuracy, half of what bf16 planes need, and 2^-e is taken off in the epilogue.  The gradient's products sum over the rows that such scales belong to, so they take three bf16 planes without
 // any, v = p0 + p1 + p2 with 24 significand bits, and the six products with i + j <= 2.  A value that is not finite is carried
 // by the first plane alone.
 constexpr float kLargest = 3.402823466e38f;
@@ -110,7 +110,7 @@ __device__ __forceinline__ void split2(float v, uint16_t* h) {
   float r = v - __half2float(a);
   if (!(fabsf(r) <= kLargest)) r = 0.f;
   h[0] = bits(a);
-  h[1] = bits(__float2half_rn(r));
+  h[1] = bits(__float2half_rn(r * (float)(1 << pg::kLowShift)));
 }
 __device__ __forceinline__ void split3(float v, uint16_t* p) {
   const __nv_bfloat16 a = __float2bfloat16_rn(v);
@@ -407,6 +407,7 @@ template <bool F32>
 struct ForwardEpi {
   static constexpr int kColumns = 128;
   static constexpr bool kDirect = false;
+  static constexpr bool kShifted = F32;
   const Head* head;
   const int* target;
   float2* part;      // [parts][n_pad]
@@ -499,6 +500,7 @@ struct GradEpi {
   // (1024 x 1024 x 16384: 120 -> 102 us), where 16-bit types lose by them (4096 x 2048 x 32000: 348 -> 361 us)
   static constexpr int kColumns = TYPE == kF32 ? 64 : 128;
   static constexpr bool kDirect = TYPE != kF32;  // (float32 dZ above: 164k cycles without, 173k with)
+  static constexpr bool kShifted = TYPE == kF32;
   const Head* head;
   const int* target;
   const float* share;
@@ -572,6 +574,7 @@ struct GradEpi {
 struct SumEpi {
   static constexpr int kColumns = 128;
   static constexpr bool kDirect = false;
+  static constexpr bool kShifted = false;
   const Head* head;
   int64_t ld;  // columns of the sums
   int add;
@@ -597,6 +600,7 @@ template <typename T>
 struct WeightEpi {
   static constexpr int kColumns = 128;
   static constexpr bool kDirect = false;
+  static constexpr bool kShifted = false;
   const Head* head;
   T* dst;
   int64_t rows, d;

@@ -4,9 +4,10 @@
 //
 // Operands are f16 or bf16 (both the same), each either k-major (rows of k) or mn-major (rows of m or n): the three
 // products of a linear layer's training step (X W^T, dZ W, dZ^T X) then read the same arrays without a transposed copy.
-// float32 operands arrive as two f16 planes (11 + 11 significand bits, scaled) or three bf16 planes (8 + 8 + 8); of the plane
-// products those with i + j <= 1, or <= 2, are summed, smallest first: the largest dropped one is 2^-22, or 2^-24, of the
-// product at most.
+// float32 operands arrive as two f16 planes (11 + 11 significand bits, scaled, the low plane by another 2^11) or three bf16 planes
+// (8 + 8 + 8); of the plane products those with i + j <= 1, or <= 2, are summed, smallest first: the largest dropped one is
+// 2^-22, or 2^-24, of the product at most.  The 2^11 is taken off the accumulator by the MMA that begins the product of the high
+// planes.
 //
 // Roles of a CTA: 4 BN / C warps drain the accumulator and run the epilogue, one issues the TMA loads of this CTA's 128 rows
 // of A and BN / 2 of the tile's BN rows of B, and the leader's last one issues the MMAs (M = 256, N = BN, K = 16) of both CTAs.  In both issuing warps all lanes run the loop and one elected lane issues, so that descriptors and addresses stay in
@@ -18,6 +19,8 @@
 // and the chunks are added there with rounding to nearest.  Two accumulators of 256 columns alternate, so the drain of one
 // runs under the MMAs of the other.
 #pragma once
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "tcgen05.cuh"
@@ -74,6 +77,16 @@ __device__ __forceinline__ void umma_f16_pair(uint32_t tmem_d, uint64_t adesc, u
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D = A B + D 2^-kLowShift
+constexpr int kLowShift = 11;
+__device__ __forceinline__ void umma_f16_pair_shifted(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.eq.u32 p, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p, %4;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "n"(kLowShift)
       : "memory");
 }
 __device__ __forceinline__ bool elect_one() {
@@ -209,8 +222,8 @@ struct Out {
 };
 
 // Epi: struct with  template <int C> __device__ void operator()(float (&acc)[C], int row, int col0, int split,
-// const CUtensorMap* tm, const Out& out)  and the constants kColumns and kDirect (below), where row and col0 are the thread's row and first of its C columns (both
-// may lie outside the result).
+// const CUtensorMap* tm, const Out& out), where row and col0 are the thread's row and first of its C columns (both may lie outside
+// the result), and the constants kColumns and kDirect (below) and kShifted (operands are two scaled planes: three products).
 template <int BN, int C, bool A_MN, bool B_MN, class Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(block_threads(BN, C), 1)
 pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -305,15 +318,17 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           ok = mbar_wait(&acc_empty[b], ((chunk >> 1) & 1) ^ 1, 22, a.dev_status, abort_flag);
           if (!ok) break;
           tc_fence_after();
-          for (int i = 0; i < steps; ++i) {
+          // (a loop of its own around the shift: with a choice in one loop the descriptors leave the uniform registers)
+          auto step = [&](int i, auto shift) {
             ok = mbar_wait(&full[s], phase, 23, a.dev_status, abort_flag);
-            if (!ok) break;
+            if (!ok) return;
             tc_fence_after();
             const uint32_t sa = smem0 + s * kStageBytes, sb = sa + kOperandBytes;
             const uint64_t da = operand_desc<A_MN>(sa), db = operand_desc<B_MN>(sb);
             if (issuer) {
+              if constexpr (decltype(shift)::value) umma_f16_pair_shifted(tmem0 + b * kTile, da, db, a.idesc);
 #pragma unroll
-              for (int k = 0; k < kBK / 16; ++k)
+              for (int k = decltype(shift)::value; k < kBK / 16; ++k)
                 umma_f16_pair(tmem0 + b * kTile, da + (uint64_t)(k * k_step_bytes<A_MN>() >> 4),
                               db + (uint64_t)(k * k_step_bytes<B_MN>() >> 4), a.idesc, k > 0 || i > 0);
               umma_commit_pair(&empty[s]);
@@ -324,7 +339,13 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               s = 0;
               phase ^= 1;
             }
+          };
+          int i = 0;
+          if constexpr (Epi::kShifted) {  // the high planes' product begins at the last third of the steps
+            for (; i < steps - (c1 - c0) && ok; ++i) step(i, std::false_type{});
+            if (ok) step(i++, std::true_type{});
           }
+          for (; i < steps && ok; ++i) step(i, std::false_type{});
         }
       }
     }

@@ -798,3 +798,21 @@ def test_a_gradient_that_is_a_negated_view(cuda):
         # the imaginary part's gradient of a conjugate: -g
         (got,) = torch.autograd.grad(torch.complex(torch.zeros_like(g), loss(leaf)).conj(), leaf, torch.complex(g, g))
         assert torch.equal(got, -want)
+
+
+@pytest.mark.parametrize("outlier", [2.0**10, 2.0**20, 2.0**24, 2.0**28])
+@pytest.mark.parametrize("n,d,v", [(200, 256, 1000), (300, 1030, 700)])
+def test_float32_rows_with_an_outlier(cuda, n, d, v, outlier):
+    """A value far above the rest of its row of X (or of W) that meets zeros of W (or X) costs the other products nothing.  A logit's operands are
+    off by 2^-22 each, the dropped product is 2^-22, values below 2^-29 of the row's largest keep 2^-50 of it, and the tensor core adds
+    48 partial sums between drains with 2^-23 each."""
+    x, w, t, up = make_ce(cuda, n, d, v, torch.float32, 0.1)
+    x[:, 3], w[:, 3] = outlier, 0
+    x[:, d - 2], w[:, d - 2] = 0, -outlier
+    loss, dx, dw = step_ce(x, w, t, up)
+    check_ce(x, w, t, up, loss, dx, dw)
+    X, W = x.double().abs(), w.double().abs()
+    X[:, 3], W[:, d - 2] = 0, 0  # (they meet zeros)
+    delta = ((48 + d / 256 + 6) * 2.0**-23 * (X @ W.t()) + 2.0**-50 * outlier * (X.sum(1, keepdim=True) + W.sum(1))).amax(1)
+    rl = reference_ce(x, w, t, up)[0]
+    assert ((loss.double() - rl).abs() <= 2 * delta + 2.0**-20 * (1 + rl.abs())).all()
