@@ -1,5 +1,5 @@
-// Cross entropy of a linear layer for few rows (one token to sixteen) where W would have to be packed for the tensor cores
-// (float32, or 16-bit rows that start anywhere): bound by the pass over W.
+// Cross entropy of a linear layer for few rows: one token to sixteen where W would have to be packed for the tensor cores (float32, or
+// 16-bit rows that start anywhere), and the forward pass of up to four rows of 16-bit types in place.  Bound by the pass over W.
 //
 // The products run on the fp32 units, in one pass: a warp takes four entries of the vocabulary at a time, its lanes go along D
 // with wide loads, one chunk ahead, and the rows of X sit in shared memory as fp32, read once for the four entries.  Forward

@@ -4,7 +4,7 @@
 //   loss = T^2 sum_k q_k (ln q_k - ln p_{i_k}),  dlogits_v = T g (p_v - sum_{k: i_k = v} q_k)
 //
 // Both directions are one pass over [N, V] and bound by HBM: forward reads it, backward reads it and writes as much
-// (4096 x 131072 bf16: 169 us, 6.4 TB/s, and 340 us, 6.3 TB/s).
+// (4096 x 131072 bf16: 160 us, 6.7 TB/s, and 344 us, 6.3 TB/s).
 //
 // Forward: a cluster of CTAs takes a row (one CTA where the rows alone fill the device, up to eight where there are few), each
 // thread keeps the running maximum and sum of its elements, the CTAs' pairs meet in the first CTA's shared memory.  The
@@ -444,7 +444,7 @@ Entries entries_of(const tcb200_topk_distill_t& p, const void* indices, const vo
 }
 
 // Threads of a CTA.  A short row is bound by its chain of loads and joins, not by its bytes: where the rows alone fill the device,
-// two warps a row keep four times as many rows in flight as eight do (8192 x 600 f16, K = 20: 32 -> 13 us forward, 23 -> 12 us
+// two warps a row keep four times as many rows in flight as eight do (8192 x 600 f16, K = 20: 32 -> 13 us forward, 23 -> 13 us
 // backward; 4096 x 8000 bf16, K = 50: 28 -> 20 and 28 -> 24).  Rows of 32 KB are better off with eight (4096 x 8000 f32 backward:
 // 58 -> 53 us), and so are many entries (8192 x 600 f16, K = 250 forward: 59 -> 47 us).
 int threads_for(const tcb200_topk_distill_t& p, int sms) {

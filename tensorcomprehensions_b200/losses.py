@@ -6,8 +6,9 @@
     logits = T.matmul(X, W)                                       # any student logits [N, V]
     loss = tc.topk_distillation(logits, indices, teacher, temperature=2.0)
 
-Both run on tensors of one CUDA device, on its current stream, without synchronising; they may be captured into CUDA graphs.
-There is no CPU or eager fallback, and no second derivative.  The reference's operator library has no loss (its tc/library ends at the layers).
+Both run on tensors of one CUDA device, on its current stream, without synchronising; they may be captured into CUDA graphs (a
+backward pass while no eager graph of the same leaves lives: torch's autograd would wait for that graph's stream, and raises).
+There is no CPU or eager fallback, no second derivative and no forward-mode one: a dual tensor raises.  The reference's operator library has no loss (its tc/library ends at the layers).
 """
 from . import tclib
 
@@ -20,8 +21,11 @@ def linear_cross_entropy(X, W, target, ignore_index=-100):
     X [N, D] and W [V, D]: float32, float16 or bfloat16, of one type, dense along D, rows any distance apart.  target [N]:
     int32 or int64.  A row with target == ignore_index has loss 0 and gradient 0, and what its X holds does not matter; a
     target outside [0, V) makes the row's loss NaN, and with it the gradients of that row of X and of W.  Gradients of
-    X and W have their type, are summed in float32 and rounded once (between the two products the gradient of z is rounded
-    to the inputs' 16-bit type; float32 inputs keep float32 accuracy throughout).  A wrong type, size, stride or device
+    X and W have their type, are summed in float32 and rounded once.  Between the two products the gradient of z is rounded to
+    the inputs' 16-bit type, relative to the batch's largest gradient of a loss (float16: rows below 2^-16 of it have a scale of
+    their own in X's gradient; W's loses what lies below 2^-39 of it).  float32 products take operands of 22 significand bits for
+    the logits, relative to a row of X or W down to 2^-29 of its largest value, and of 24 for the gradients: float32 accuracy.
+    If a wait inside a kernel gives up (never on a sound device), the loss, or both gradients, are NaN.  A wrong type, size, stride or device
     raises RuntimeError."""
     return tclib.linear_cross_entropy(X, W, target, ignore_index)
 
