@@ -249,7 +249,8 @@ enum { TCB200_F32 = 0, TCB200_F16 = 1, TCB200_BF16 = 2 };
  *   lse[n] = log sum_v exp z(n,v),  loss[n] = lse[n] - z(n, target[n]),
  *   dX = dZ W, dW = dZ^T X  with  dZ(n,v) = grad_loss[n] (exp(z(n,v) - lse[n]) - [v = target[n]]).
  * target[n] == ignore_index: loss, lse and the row of dX are 0, the row of X is not read.  A target outside [0, V) that is
- * not ignore_index makes loss[n], the row of dX and all of dW NaN. */
+ * not ignore_index makes loss[n], the row of dX and all of dW NaN.  f16 and bf16: dZ is rounded to the type between the two
+ * products of the gradient, relative to the largest |grad_loss| (f16: rows below 2^-16 of it have a scale of their own in dX). */
 typedef struct tcb200_linear_ce {
   int64_t N, D, V;         /* X is [N, D], W is [V, D], target, loss and lse are [N] */
   int64_t ldx, ldw;        /* elements between rows of X and of W (>= D); dX and dW are dense */
